@@ -26,6 +26,18 @@ except ImportError as exc:  # pragma: no cover - depends on the build state
 if not _BUILDING or "feather_ops_b200._C" in sys.modules:
     from .conv2d import conv3x3_prepacked, prepack_conv2d_weight_3x3
     from .conv2d_module import Conv2d
+    from .fp8_block import (
+        dequantize_fp8_weight,
+        fp8_block_dgrad,
+        fp8_block_linear,
+        fp8_block_mm,
+        quantize_fp8_activation,
+        quantize_fp8_weight,
+        rms_norm_dgrad,
+        rms_norm_quantize_fp8,
+        silu_mul_dgrad,
+        silu_mul_quantize_fp8,
+    )
     from .int8_convrot import (
         convrot_int8_dgrad,
         convrot_int8_linear,
@@ -45,6 +57,10 @@ if not _BUILDING or "feather_ops_b200._C" in sys.modules:
         "convrot_int8_dgrad",
         "convrot_int8_linear",
         "dequantize_convrot_weight",
+        "dequantize_fp8_weight",
+        "fp8_block_dgrad",
+        "fp8_block_linear",
+        "fp8_block_mm",
         "int8_scaled_mm",
         "int8_scaled_mm_plain",
         "prepack_b_for_scaled_mm",
@@ -52,6 +68,12 @@ if not _BUILDING or "feather_ops_b200._C" in sys.modules:
         "prepack_int8_weight",
         "quantize_convrot_activation",
         "quantize_convrot_weight",
+        "quantize_fp8_activation",
+        "quantize_fp8_weight",
+        "rms_norm_dgrad",
+        "rms_norm_quantize_fp8",
         "scaled_mm_hip",
+        "silu_mul_dgrad",
+        "silu_mul_quantize_fp8",
         "unpack_int8_weight",
     ]

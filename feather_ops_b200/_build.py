@@ -32,6 +32,8 @@ KERNEL_SOURCES = [
     "convrot_quantize_sm100.cu",
     "int8_mm_sm100.cu",
     "conv3x3_sm100.cu",
+    "fp8_block_quantize_sm100.cu",
+    "fp8_block_mm_sm100.cu",
     "selftest_sm100.cu",
 ]
 NVCC_FLAGS = [

@@ -53,6 +53,13 @@ PROTOTYPES = {
         [_ptr, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _ptr],
     ),
     "feather_conv3x3_status": (_c_int, [_ptr]),
+    "launch_fp8_block_quantize": (_c_bool, [_ptr, _ptr, _ptr, _i64, _i64, _c_int, _c_int, _ptr]),
+    "launch_fp8_block_mm": (_c_bool, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _c_bool, _c_int, _c_int, _c_int, _ptr]),
+    "launch_rms_norm_fp8": (_c_bool, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, ctypes.c_float, _c_int, _c_int, _c_int, _ptr]),
+    "launch_rms_norm_dgrad": (_c_bool, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _c_int, _c_int, _ptr]),
+    "feather_rms_norm_dgrad_partial_floats": (_i64, [_i64, _i64]),
+    "launch_silu_mul_fp8": (_c_bool, [_ptr, _ptr, _ptr, _i64, _i64, _c_int, _c_int, _ptr]),
+    "launch_silu_mul_dgrad": (_c_bool, [_ptr, _ptr, _ptr, _i64, _i64, _c_int, _ptr]),
     "feather_selftest_wait_runs_out": (_c_int, [ctypes.c_longlong, _ptr, _ptr, _ptr]),
 }
 

@@ -1,7 +1,7 @@
 // Thin torch extension over the C ABI: registers the `torch.ops.feather_ops.*` operators: four with the
 // schemas of the reference (csrc/hip_kernel.cu:825-846, csrc/hip_kernel_int8.cu:564-586 and :972-980,
-// csrc/hip_conv2d_3x3.cu:672-692) and `scaled_mm_splitk` (the skinny-M launcher over caller scratch, no
-// counterpart in the reference). It validates tensors with the reference's messages, takes the current
+// csrc/hip_conv2d_3x3.cu:672-692), `scaled_mm_splitk` (the skinny-M launcher over caller scratch) and the block-scaled
+// fp8 operators (neither has a counterpart in the reference). It validates tensors with the reference's messages, takes the current
 // CUDA stream of the input's device and forwards raw pointers to libfeather_ops_b200.so. Built against
 // torch's stable ABI, so it does not depend on libtorch_python. Nothing here computes or allocates.
 #include <Python.h>
@@ -319,6 +319,173 @@ void convrot_quantize(const Tensor& x, const std::optional<Tensor>& col_scale, T
     STD_TORCH_CHECK(ok, "convrot_quantize launch failed");
 }
 
+bool is_fp8(ScalarType t) { return t == ScalarType::Float8_e4m3fn || t == ScalarType::Float8_e5m2; }
+
+// The block-scaled fp8 operators (no counterpart in the reference). `scale` of an activation is [ceil(K / 128), M].
+void check_block_codes(const Tensor& q, const Tensor& scale, int64_t M, int64_t K, int32_t device) {
+    STD_TORCH_CHECK(q.is_cuda() && scale.is_cuda() && q.get_device_index() == device && scale.get_device_index() == device,
+                    "the codes and their scales must be on the input's CUDA device");
+    STD_TORCH_CHECK(is_fp8(q.scalar_type()), "the codes must be float8_e4m3fn or float8_e5m2");
+    STD_TORCH_CHECK(scale.scalar_type() == ScalarType::Float, "the block scales must be float32");
+    STD_TORCH_CHECK(K > 0 && K % 16 == 0, "the row length must be a positive multiple of 16");
+    STD_TORCH_CHECK(q.dim() == 2 && q.size(0) == M && q.size(1) == K, "the codes must be [", M, ", ", K, "]");
+    STD_TORCH_CHECK(scale.dim() == 2 && scale.size(0) == (K + 127) / 128 && scale.size(1) == M, "the block scales must be [", (K + 127) / 128, ", ", M, "]");
+    STD_TORCH_CHECK(q.is_contiguous() && scale.is_contiguous(), "the codes and their scales must be contiguous");
+    STD_TORCH_CHECK(aligned16(q.const_data_ptr()), "the codes' data pointer must be 16-byte aligned");
+}
+
+// A 16-bit matrix [M, K] that a row-wise kernel reads or writes, of dtype `type` on `device`.
+void check_rows(const Tensor& t, const char* name, int64_t M, int64_t K, ScalarType type, int32_t device) {
+    STD_TORCH_CHECK(t.is_cuda() && t.get_device_index() == device, name, " must be on the input's CUDA device");
+    STD_TORCH_CHECK(t.scalar_type() == type, name, " must have the input's dtype");
+    STD_TORCH_CHECK(t.dim() == 2 && t.size(0) == M && t.size(1) == K, name, " must be [", M, ", ", K, "]");
+    STD_TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+    STD_TORCH_CHECK(aligned16(t.const_data_ptr()), name, " data pointer must be 16-byte aligned");
+}
+
+void fp8_block_quantize(const Tensor& x, Tensor& q, Tensor& scale) {
+    STD_TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+    STD_TORCH_CHECK(is_half_or_bf16(x.scalar_type()), "x must be float16 or bfloat16");
+    STD_TORCH_CHECK(x.dim() == 2, "x must be 2D");
+    const auto device = x.get_device_index();
+    const int64_t M = x.size(0), K = x.size(1);
+    check_rows(x, "x", M, K, x.scalar_type(), device);
+    check_block_codes(q, scale, M, K, device);
+    torch::stable::accelerator::DeviceGuard guard(device);
+    const bool ok = launch_fp8_block_quantize(x.const_data_ptr(), q.mutable_data_ptr(), static_cast<float*>(scale.mutable_data_ptr()), M, K,
+                                              x.scalar_type() == ScalarType::Half ? 1 : 0, q.scalar_type() == ScalarType::Float8_e5m2 ? 1 : 0,
+                                              current_stream(device));
+    STD_TORCH_CHECK(ok, "fp8_block_quantize launch failed");
+}
+
+void fp8_block_mm(const Tensor& a, const Tensor& a_scale, const Tensor& weight, const Tensor& weight_scale, const std::optional<Tensor>& bias, Tensor& c,
+                  bool transposed_b) {
+    STD_TORCH_CHECK(a.is_cuda() && weight.is_cuda() && weight_scale.is_cuda() && c.is_cuda(), "tensors must be CUDA tensors");
+    const auto device = a.get_device_index();
+    STD_TORCH_CHECK(weight.get_device_index() == device && weight_scale.get_device_index() == device && c.get_device_index() == device,
+                    "tensors must be on the same device");
+    STD_TORCH_CHECK(is_fp8(weight.scalar_type()), "weight must be float8_e4m3fn or float8_e5m2");
+    STD_TORCH_CHECK(is_half_or_bf16(c.scalar_type()), "c must be float16 or bfloat16");
+    STD_TORCH_CHECK(a.dim() == 2 && weight.dim() == 2 && c.dim() == 2, "a, weight and c must be 2D");
+    const int64_t M = a.size(0), N = weight.size(0), K = weight.size(1);
+    STD_TORCH_CHECK(N > 0 && K > 0 && N % 16 == 0 && K % 16 == 0, "the weight axes must be positive multiples of 16");
+    STD_TORCH_CHECK(a.size(1) == (transposed_b ? N : K), "a's row length must equal the weight axis that is contracted");
+    check_block_codes(a, a_scale, M, a.size(1), device);
+    STD_TORCH_CHECK(weight_scale.scalar_type() == ScalarType::Float, "weight_scale must be float32");
+    STD_TORCH_CHECK(weight_scale.dim() == 2 && weight_scale.size(0) == (N + 127) / 128 && weight_scale.size(1) == (K + 127) / 128,
+                    "weight_scale must be [", (N + 127) / 128, ", ", (K + 127) / 128, "]");
+    STD_TORCH_CHECK(c.size(0) == M && c.size(1) == (transposed_b ? K : N), "c has the wrong shape");
+    STD_TORCH_CHECK(weight.is_contiguous() && weight_scale.is_contiguous() && c.is_contiguous(), "weight, weight_scale and c must be contiguous");
+    STD_TORCH_CHECK(!transposed_b || !bias.has_value(), "transposed_b takes no bias");
+    if (bias.has_value()) {
+        STD_TORCH_CHECK(bias->is_cuda() && bias->scalar_type() == c.scalar_type() && bias->get_device_index() == device, "bias must have c's dtype and device");
+        STD_TORCH_CHECK(bias->numel() == N && bias->is_contiguous(), "bias must have N contiguous elements");
+    }
+    STD_TORCH_CHECK(aligned16(weight.const_data_ptr()) && aligned16(c.mutable_data_ptr()), "data pointers must be 16-byte aligned");
+    torch::stable::accelerator::DeviceGuard guard(device);
+    const bool ok = launch_fp8_block_mm(
+        static_cast<const uint8_t*>(a.const_data_ptr()), static_cast<const float*>(a_scale.const_data_ptr()), static_cast<const uint8_t*>(weight.const_data_ptr()),
+        static_cast<const float*>(weight_scale.const_data_ptr()), bias.has_value() ? static_cast<const uint16_t*>(bias->const_data_ptr()) : nullptr,
+        static_cast<uint16_t*>(c.mutable_data_ptr()), M, N, K, transposed_b, a.scalar_type() == ScalarType::Float8_e5m2 ? 1 : 0,
+        weight.scalar_type() == ScalarType::Float8_e5m2 ? 1 : 0, c.scalar_type() == ScalarType::Half ? 0 : 1, current_stream(device));
+    STD_TORCH_CHECK(ok, "fp8_block_mm launch failed");
+}
+
+// The norm's weight: [K], of the input's dtype or float32.
+void check_norm_weight(const Tensor& weight, const Tensor& x, int64_t K) {
+    STD_TORCH_CHECK(weight.is_cuda() && weight.get_device_index() == x.get_device_index(), "weight must be on the input's CUDA device");
+    STD_TORCH_CHECK(weight.scalar_type() == x.scalar_type() || weight.scalar_type() == ScalarType::Float, "weight must have the input's dtype or be float32");
+    STD_TORCH_CHECK(weight.dim() == 1 && weight.size(0) == K, "weight must be [", K, "]");
+    STD_TORCH_CHECK(weight.is_contiguous() && aligned16(weight.const_data_ptr()), "weight must be contiguous and 16-byte aligned");
+    STD_TORCH_CHECK(K <= 32768, "a norm's rows may have at most 32768 channels");
+}
+
+void rms_norm_fp8(const Tensor& x, const std::optional<Tensor>& residual, const Tensor& weight, const std::optional<Tensor>& residual_out, Tensor& q,
+                  Tensor& scale, Tensor& rstd, double eps) {
+    STD_TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+    STD_TORCH_CHECK(is_half_or_bf16(x.scalar_type()), "x must be float16 or bfloat16");
+    STD_TORCH_CHECK(x.dim() == 2, "x must be 2D");
+    const auto device = x.get_device_index();
+    const int64_t M = x.size(0), K = x.size(1);
+    check_rows(x, "x", M, K, x.scalar_type(), device);
+    STD_TORCH_CHECK(residual.has_value() == residual_out.has_value(), "residual and residual_out come together");
+    if (residual.has_value()) {
+        check_rows(*residual, "residual", M, K, x.scalar_type(), device);
+        check_rows(*residual_out, "residual_out", M, K, x.scalar_type(), device);
+    }
+    check_block_codes(q, scale, M, K, device);
+    check_norm_weight(weight, x, K);
+    STD_TORCH_CHECK(rstd.is_cuda() && rstd.get_device_index() == device && rstd.scalar_type() == ScalarType::Float && rstd.numel() == M && rstd.is_contiguous(),
+                    "rstd must be M contiguous float32 on the input's device");
+    STD_TORCH_CHECK(eps >= 0, "eps must not be negative");
+    torch::stable::accelerator::DeviceGuard guard(device);
+    const bool ok = launch_rms_norm_fp8(x.const_data_ptr(), residual.has_value() ? residual->const_data_ptr() : nullptr, weight.const_data_ptr(),
+                                        residual_out.has_value() ? residual_out->mutable_data_ptr() : nullptr, q.mutable_data_ptr(),
+                                        static_cast<float*>(scale.mutable_data_ptr()), static_cast<float*>(rstd.mutable_data_ptr()), M, K, static_cast<float>(eps),
+                                        x.scalar_type() == ScalarType::Half ? 1 : 0, weight.scalar_type() == ScalarType::Float ? 1 : 0,
+                                        q.scalar_type() == ScalarType::Float8_e5m2 ? 1 : 0, current_stream(device));
+    STD_TORCH_CHECK(ok, "rms_norm_fp8 launch failed");
+}
+
+void rms_norm_dgrad(const Tensor& grad, const Tensor& x, const Tensor& weight, const Tensor& rstd, const std::optional<Tensor>& grad_residual, Tensor& grad_x,
+                    Tensor& grad_weight, Tensor& partials) {
+    STD_TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+    STD_TORCH_CHECK(is_half_or_bf16(x.scalar_type()), "x must be float16 or bfloat16");
+    STD_TORCH_CHECK(x.dim() == 2, "x must be 2D");
+    const auto device = x.get_device_index();
+    const int64_t M = x.size(0), K = x.size(1);
+    STD_TORCH_CHECK(M > 0 && K > 0 && K % 16 == 0, "x must have rows, and a row length that is a positive multiple of 16");
+    check_rows(x, "x", M, K, x.scalar_type(), device);
+    check_rows(grad, "grad", M, K, x.scalar_type(), device);
+    if (grad_residual.has_value()) check_rows(*grad_residual, "grad_residual", M, K, x.scalar_type(), device);
+    check_rows(grad_x, "grad_x", M, K, x.scalar_type(), device);
+    check_norm_weight(weight, x, K);
+    STD_TORCH_CHECK(rstd.is_cuda() && rstd.get_device_index() == device && rstd.scalar_type() == ScalarType::Float && rstd.numel() == M && rstd.is_contiguous(),
+                    "rstd must be M contiguous float32 on the input's device");
+    STD_TORCH_CHECK(grad_weight.is_cuda() && grad_weight.get_device_index() == device && grad_weight.scalar_type() == ScalarType::Float &&
+                        grad_weight.numel() == K && grad_weight.is_contiguous(),
+                    "grad_weight must be K contiguous float32 on the input's device");
+    torch::stable::accelerator::DeviceGuard guard(device);
+    STD_TORCH_CHECK(partials.is_cuda() && partials.get_device_index() == device && partials.scalar_type() == ScalarType::Float && partials.is_contiguous() &&
+                        partials.numel() >= feather_rms_norm_dgrad_partial_floats(M, K) && aligned16(partials.const_data_ptr()),
+                    "partials must be contiguous float32 scratch of the size feather_rms_norm_dgrad_partial_floats gives");
+    const bool ok = launch_rms_norm_dgrad(grad.const_data_ptr(), x.const_data_ptr(), weight.const_data_ptr(), static_cast<const float*>(rstd.const_data_ptr()),
+                                          grad_residual.has_value() ? grad_residual->const_data_ptr() : nullptr, grad_x.mutable_data_ptr(),
+                                          static_cast<float*>(grad_weight.mutable_data_ptr()), static_cast<float*>(partials.mutable_data_ptr()), M, K,
+                                          x.scalar_type() == ScalarType::Half ? 1 : 0, weight.scalar_type() == ScalarType::Float ? 1 : 0, current_stream(device));
+    STD_TORCH_CHECK(ok, "rms_norm_dgrad launch failed");
+}
+
+void silu_mul_fp8(const Tensor& gate_up, Tensor& q, Tensor& scale) {
+    STD_TORCH_CHECK(gate_up.is_cuda(), "gate_up must be a CUDA tensor");
+    STD_TORCH_CHECK(is_half_or_bf16(gate_up.scalar_type()), "gate_up must be float16 or bfloat16");
+    STD_TORCH_CHECK(gate_up.dim() == 2 && gate_up.size(1) % 2 == 0, "gate_up must be [M, 2 F]");
+    const auto device = gate_up.get_device_index();
+    const int64_t M = gate_up.size(0), F = gate_up.size(1) / 2;
+    check_rows(gate_up, "gate_up", M, 2 * F, gate_up.scalar_type(), device);
+    check_block_codes(q, scale, M, F, device);
+    torch::stable::accelerator::DeviceGuard guard(device);
+    const bool ok = launch_silu_mul_fp8(gate_up.const_data_ptr(), q.mutable_data_ptr(), static_cast<float*>(scale.mutable_data_ptr()), M, F,
+                                        gate_up.scalar_type() == ScalarType::Half ? 1 : 0, q.scalar_type() == ScalarType::Float8_e5m2 ? 1 : 0,
+                                        current_stream(device));
+    STD_TORCH_CHECK(ok, "silu_mul_fp8 launch failed");
+}
+
+void silu_mul_dgrad(const Tensor& grad, const Tensor& gate_up, Tensor& grad_gate_up) {
+    STD_TORCH_CHECK(gate_up.is_cuda(), "gate_up must be a CUDA tensor");
+    STD_TORCH_CHECK(is_half_or_bf16(gate_up.scalar_type()), "gate_up must be float16 or bfloat16");
+    STD_TORCH_CHECK(gate_up.dim() == 2 && gate_up.size(1) > 0 && gate_up.size(1) % 32 == 0, "gate_up must be [M, 2 F], F a positive multiple of 16");
+    const auto device = gate_up.get_device_index();
+    const int64_t M = gate_up.size(0), F = gate_up.size(1) / 2;
+    check_rows(gate_up, "gate_up", M, 2 * F, gate_up.scalar_type(), device);
+    check_rows(grad, "grad", M, F, gate_up.scalar_type(), device);
+    check_rows(grad_gate_up, "grad_gate_up", M, 2 * F, gate_up.scalar_type(), device);
+    torch::stable::accelerator::DeviceGuard guard(device);
+    const bool ok = launch_silu_mul_dgrad(grad.const_data_ptr(), gate_up.const_data_ptr(), grad_gate_up.mutable_data_ptr(), M, F,
+                                          gate_up.scalar_type() == ScalarType::Half ? 1 : 0, current_stream(device));
+    STD_TORCH_CHECK(ok, "silu_mul_dgrad launch failed");
+}
+
 void conv2d_3x3(const Tensor& x, const Tensor& w_prepacked, const std::optional<Tensor>& bias, Tensor& out, int64_t warps_m, int64_t warps_n,
                 int64_t repeat_m, int64_t repeat_n, int64_t rows, bool prefetch) {
     STD_TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
@@ -392,6 +559,17 @@ STABLE_TORCH_LIBRARY(feather_ops, m) {
         "int block_warps_m, int block_warps_n, int unroll_k, int repeat_m, int repeat_n) -> ()");
     m.def("int8_scaled_mm_plain(Tensor a, Tensor weight, Tensor a_scale, Tensor? b_scale, Tensor? bias, Tensor(a!) c, bool transposed_b) -> ()");
     m.def("convrot_quantize(Tensor x, Tensor? col_scale, Tensor(a!) q, Tensor(b!) row_scale, bool rotate) -> ()");
+    m.def("fp8_block_quantize(Tensor x, Tensor(a!) q, Tensor(b!) scale) -> ()");
+    m.def(
+        "fp8_block_mm(Tensor a, Tensor a_scale, Tensor weight, Tensor weight_scale, Tensor? bias, Tensor(a!) c, bool transposed_b) -> ()");
+    m.def(
+        "rms_norm_fp8(Tensor x, Tensor? residual, Tensor weight, Tensor(a!)? residual_out, Tensor(b!) q, Tensor(c!) scale, Tensor(d!) rstd, "
+        "float eps) -> ()");
+    m.def(
+        "rms_norm_dgrad(Tensor grad, Tensor x, Tensor weight, Tensor rstd, Tensor? grad_residual, Tensor(a!) grad_x, Tensor(b!) grad_weight, "
+        "Tensor(c!) partials) -> ()");
+    m.def("silu_mul_fp8(Tensor gate_up, Tensor(a!) q, Tensor(b!) scale) -> ()");
+    m.def("silu_mul_dgrad(Tensor grad, Tensor gate_up, Tensor(a!) grad_gate_up) -> ()");
     m.def(
         "conv2d_3x3(Tensor x, Tensor w_prepacked, Tensor? bias, Tensor(a!) out, int warps_m, int warps_n, int repeat_m, int repeat_n, "
         "int rows, bool prefetch) -> ()");
@@ -404,6 +582,12 @@ STABLE_TORCH_LIBRARY_IMPL(feather_ops, CUDA, m) {
     m.impl("int8_scaled_mm", TORCH_BOX(&int8_scaled_mm));
     m.impl("int8_scaled_mm_plain", TORCH_BOX(&int8_scaled_mm_plain));
     m.impl("convrot_quantize", TORCH_BOX(&convrot_quantize));
+    m.impl("fp8_block_quantize", TORCH_BOX(&fp8_block_quantize));
+    m.impl("fp8_block_mm", TORCH_BOX(&fp8_block_mm));
+    m.impl("rms_norm_fp8", TORCH_BOX(&rms_norm_fp8));
+    m.impl("rms_norm_dgrad", TORCH_BOX(&rms_norm_dgrad));
+    m.impl("silu_mul_fp8", TORCH_BOX(&silu_mul_fp8));
+    m.impl("silu_mul_dgrad", TORCH_BOX(&silu_mul_dgrad));
     m.impl("conv2d_3x3", TORCH_BOX(&conv2d_3x3));
 }
 

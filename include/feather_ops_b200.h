@@ -147,6 +147,43 @@ int feather_conv3x3_launch(const void* x, const void* wp, const void* bias, void
 /* Diagnostic for the conv kernel's bounded waits, as feather_scaled_mm_status. No counterpart in the reference. */
 int feather_conv3x3_status(uint32_t* out);
 
+/* fp8 codes of an activation with one float32 scale per row and 128 channels: with t = max(max |x| over the block, 1e-30 top) and
+ * top = 448 (e4m3) or 57344 (e5m2), scale = t / top and q = fp8(x * (top / t)). x: [M, K] fp16 (input_fp16 != 0) or bf16; q: [M, K];
+ * scale: [ceil(K / 128), M]. K % 16 == 0, x and q 16-byte aligned. No counterpart in the reference (its quantizer is per row, to int8,
+ * csrc/hip_kernel_int8.cu:869-878). */
+bool launch_fp8_block_quantize(const void* x, void* q, float* scale, int64_t M, int64_t K, int input_fp16, int use_e5m2, feather_stream_t stream);
+
+/* fp8 x fp8 product with block scales, w = [N, K] codes row-major, w_scale = [ceil(N / 128), ceil(K / 128)], float32 accumulation:
+ * forward (transposed_b false): c[M, N] = sum over blocks b of K of a_scale[b][m] w_scale[n / 128][b] (a[m, b] . w[n, b]) + bias[n];
+ * backward (transposed_b true): c[M, K] = sum over blocks b of N of a_scale[b][m] w_scale[b][k / 128] (a[m, b] . w[b, k]), bias NULL.
+ * a: [M, K] (backward [M, N]) codes, a_scale: [ceil(contraction / 128), M] as launch_fp8_block_quantize writes it. a_e5m2 / w_e5m2: the
+ * codes' type (0 = e4m3). output_dtype of c and bias: 0 = fp16, 1 = bf16. N % 16 == 0, K % 16 == 0; a, w and c 16-byte aligned.
+ * Returns false for bad arguments. No counterpart in the reference. */
+bool launch_fp8_block_mm(const uint8_t* a, const float* a_scale, const uint8_t* w, const float* w_scale, const uint16_t* bias, uint16_t* c, int64_t M,
+                         int64_t N, int64_t K, bool transposed_b, int a_e5m2, int w_e5m2, int output_dtype, feather_stream_t stream);
+
+/* RMS norm with its output in fp8: h = x + residual rounded to the input's type (h = x without a residual), rstd = 1 / sqrt(mean(h^2) + eps),
+ * and the codes and scales of h * rstd * weight as launch_fp8_block_quantize gives them. x, residual, residual_out (= h): [M, K], fp16 or bf16;
+ * residual and residual_out both NULL without a residual. weight: [K] of x's type or float32 (weight_f32 != 0). rstd: [M] float32.
+ * K % 16 == 0, K <= 32768, every matrix and the weight 16-byte aligned, no output overlaps an input. No counterpart in the reference. */
+bool launch_rms_norm_fp8(const void* x, const void* residual, const void* weight, void* residual_out, void* q, float* scale, float* rstd, int64_t M,
+                         int64_t K, float eps, int input_fp16, int weight_f32, int use_e5m2, feather_stream_t stream);
+
+/* Backward pass of the norm: with n = x rstd (x: what the norm was taken of, i.e. residual_out where there was a residual) and
+ * u = grad * weight, grad_x = rstd (u - n mean(u n)) + grad_residual, grad_weight = sum over rows of grad * n (float32, the same bits on
+ * every run of one device). grad_residual: [M, K] or NULL. partials: feather_rms_norm_dgrad_partial_floats(M, K) floats of scratch, 16-byte
+ * aligned. M >= 1, the norm's other conditions. No counterpart in the reference. */
+bool launch_rms_norm_dgrad(const void* grad, const void* x, const void* weight, const float* rstd, const void* grad_residual, void* grad_x,
+                           float* grad_weight, float* partials, int64_t M, int64_t K, int input_fp16, int weight_f32, feather_stream_t stream);
+int64_t feather_rms_norm_dgrad_partial_floats(int64_t M, int64_t K);
+
+/* Codes and scales (as launch_fp8_block_quantize) of silu(gate) * up, gate_up = [M, 2 F] with the gate's columns first. q: [M, F], scale:
+ * [ceil(F / 128), M]. F % 16 == 0, matrices 16-byte aligned. No counterpart in the reference. */
+bool launch_silu_mul_fp8(const void* gate_up, void* q, float* scale, int64_t M, int64_t F, int input_fp16, int use_e5m2, feather_stream_t stream);
+
+/* Gradient of gate_up [M, 2 F] from grad [M, F], the gradient of silu(gate) * up; one 16-bit type for all three. No counterpart in the reference. */
+bool launch_silu_mul_dgrad(const void* grad, const void* gate_up, void* grad_gate_up, int64_t M, int64_t F, int input_fp16, feather_stream_t stream);
+
 /* Self-test of the bounded device waits every tcgen05 kernel here is built on: one warp waits, for at most limit_cycles
  * SM clocks (clamped to [1e5, 4e9]), on a barrier that nothing arrives on, gives up, records it and the kernel ends
  * normally; a second waiter with a 64 times longer limit must leave through the abort flag. Synchronizes `stream`.
