@@ -250,6 +250,29 @@ __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64
         : "memory");
 }
 
+// D[tmem] (+)= A[smem] * B[smem], 8-bit floating point operands (each side e4m3 or e5m2, by the descriptor), fp32 accumulate.
+__device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+        "}\n"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// 32 lanes x 16 consecutive 32-bit columns
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
+
 // 32 lanes x 32 consecutive 32-bit columns: thread `lane` of the warp gets row (lane) of its lane quarter.
 __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t (&v)[32]) {
     asm volatile(
@@ -291,6 +314,10 @@ __device__ __forceinline__ uint32_t map_to_cta(uint32_t local, uint32_t rank) {
 // 16 bytes into another CTA's shared memory (distributed shared memory; the address comes from map_to_cta)
 __device__ __forceinline__ void st_shared_cluster_v4(uint32_t cluster_addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
     asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+__device__ __forceinline__ void st_shared_cluster_f32(uint32_t cluster_addr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
 }
 
 // Arrive on a barrier given by its shared::cluster address (this CTA's or the peer's). Plain release
@@ -339,6 +366,28 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t desc_a, u
         : "memory");
 }
 
+__device__ __forceinline__ void umma_f8_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+        "}\n"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Moves registers between the warpgroups of a CTA: all four warps of a group execute it, and the groups' shares together
+// stay within the CTA's registers at launch (an increase waits for them).
+template <int kRegisters>
+__device__ __forceinline__ void registers_decrease() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegisters));
+}
+template <int kRegisters>
+__device__ __forceinline__ void registers_increase() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegisters));
+}
+
 // ---------------------------------------------------------------------------------------------------------
 // Descriptors
 // ---------------------------------------------------------------------------------------------------------
@@ -348,6 +397,8 @@ constexpr uint32_t kFmtF16 = 0;   // kind::f16 operand formats
 constexpr uint32_t kFmtBF16 = 1;
 constexpr uint32_t kFmtU8 = 0;    // kind::i8 operand formats
 constexpr uint32_t kFmtS8 = 1;
+constexpr uint32_t kFmtE4M3 = 0;  // kind::f8f6f4 operand formats
+constexpr uint32_t kFmtE5M2 = 1;
 constexpr uint32_t kAccF32 = 1;
 constexpr uint32_t kAccS32 = 2;
 
@@ -381,6 +432,7 @@ __device__ __forceinline__ uint64_t make_desc_sw128_kmajor(uint32_t smem_addr) {
 __device__ __forceinline__ uint64_t make_desc_sw128_mnmajor(uint32_t smem_addr) {
     return make_smem_desc(smem_addr, 16u, 1024u, kSwizzle128B);
 }
+constexpr uint32_t kIdescAMajorMN = 1u << 15;
 constexpr uint32_t kIdescBMajorMN = 1u << 16;
 
 // Tile walk of the persistent pair kernels: row tiles fastest inside a band of `band` row tiles, all column tiles

@@ -162,6 +162,9 @@ bool launch_fp8_block_quantize(const void* x, void* q, float* scale, int64_t M, 
 bool launch_fp8_block_mm(const uint8_t* a, const float* a_scale, const uint8_t* w, const float* w_scale, const uint16_t* bias, uint16_t* c, int64_t M,
                          int64_t N, int64_t K, bool transposed_b, int a_e5m2, int w_e5m2, int output_dtype, feather_stream_t stream);
 
+/* Diagnostic for the block-scaled product's bounded waits, as feather_scaled_mm_status. No counterpart in the reference. */
+int feather_fp8_block_mm_status(uint32_t* out);
+
 /* RMS norm with its output in fp8: h = x + residual rounded to the input's type (h = x without a residual), rstd = 1 / sqrt(mean(h^2) + eps),
  * and the codes and scales of h * rstd * weight as launch_fp8_block_quantize gives them. x, residual, residual_out (= h): [M, K], fp16 or bf16;
  * residual and residual_out both NULL without a residual. weight: [K] of x's type or float32 (weight_f32 != 0). rstd: [M] float32.

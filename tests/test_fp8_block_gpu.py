@@ -9,6 +9,7 @@ import pytest
 import torch
 
 import feather_ops_b200 as fo
+from feather_ops_b200 import _lib
 from oracle import fp8_block as ofb
 
 pytestmark = pytest.mark.gpu
@@ -16,6 +17,12 @@ pytestmark = pytest.mark.gpu
 E4M3, E5M2 = torch.float8_e4m3fn, torch.float8_e5m2
 HALF = {torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11}   # half a step relative to the value
 TINY = {torch.bfloat16: 2.0**-133, torch.float16: 2.0**-25}  # half a step of the smallest numbers
+
+
+@pytest.fixture(autouse=True)
+def every_wait_completed(cuda_device):
+    yield
+    assert _lib.read_status("feather_fp8_block_mm_status") == (0, 0)
 
 
 def _rand(rows, width, dtype, seed, size=1.0):
@@ -87,7 +94,7 @@ def test_quantizer_extremes(cuda_device, dtype):
 SHAPES = [
     (1, 16, 16), (1, 512, 4096), (2, 4096, 512), (7, 272, 400), (8, 1040, 1296), (16, 128, 128), (17, 256, 2064), (24, 5120, 1280), (33, 144, 3856),
     (63, 528, 640), (64, 2048, 2048), (65, 400, 272), (100, 1296, 768), (127, 112, 256), (128, 128, 1024), (129, 272, 144), (200, 1280, 5120),
-    (255, 640, 528), (256, 256, 256), (257, 768, 272), (300, 2576, 1040), (511, 384, 2576), (777, 3856, 400), (1030, 272, 1296), (2100, 1552, 656),
+    (255, 640, 528), (256, 256, 256), (257, 768, 272), (300, 2576, 1040), (511, 384, 2576), (777, 3856, 400), (1030, 272, 1296), (2100, 1552, 656), (777, 400, 3856), (2600, 272, 1040),
 ]
 
 
