@@ -84,9 +84,18 @@ __device__ __forceinline__ uint32_t pack_out(float a, float b) {
     }
 }
 
-// Every lane waits; the warp goes on together or not at all.
+// The warp goes on together or not at all. The first poll is everybody's; a barrier that is not there yet is left to one
+// lane, whose polls do not crowd the shared memory that the UMMAs read their operands from.
+__device__ __forceinline__ bool warp_wait_longer(const WaitGuard& guard, uint64_t* bar, uint32_t parity, uint32_t site) {
+    bool ok = true;
+    if (threadIdx.x % 32 == 0) ok = guard.wait(bar, parity, site);
+    return __shfl_sync(0xffffffffu, ok, 0);
+}
+
 __device__ __forceinline__ bool warp_wait(const WaitGuard& guard, uint64_t* bar, uint32_t parity, uint32_t site) {
-    return __all_sync(0xffffffffu, guard.wait(bar, parity, site));
+    const bool ok = __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || warp_wait_longer(guard, bar, parity, site);
+    __syncwarp();
+    return ok;
 }
 
 // A wait has run out somewhere in the CTA: copies in flight get time to land before the CTA gives up its shared memory.
@@ -98,30 +107,76 @@ __device__ __forceinline__ void let_copies_land(const WaitGuard& guard) {
     }
 }
 
+// Scales. A load into a register that is used some k blocks later does not work: the loads of all the k blocks in between
+// share the warp's few scoreboards, so the first use waits for the newest of them (3 loads per k block, fetched four ahead,
+// cost the pair kernel 200 of 620 us at 8192 x 12288 x 4096). So one warp brings the scales of k block after k block into
+// shared memory with asynchronous copies, kAhead blocks early, and writes the products sa * sw for the epilogue warps. Its
+// arrival is the second one on the accumulator's "full" barrier, so the epilogue waits for both at once.
+constexpr int kScaleAhead = 6;
+constexpr int kScaleRing = 8;   // raw scales: more than kScaleAhead, a lane may still read the one before
+
+// [kRows activation scales (zeros from `live` on), two weight scales] into `raw`
+template <int kRows>
+__device__ __forceinline__ void fetch_scales(float* raw, const float* a_scale, int live, const float* w0, const float* w1) {
+    const int lane = static_cast<int>(threadIdx.x) % 32;
+    const uint32_t to = smem_u32(raw);
+#pragma unroll
+    for (int r = lane; r < kRows; r += 32) cp_async_4(to + r * 4, r < live ? a_scale + r : a_scale, r < live);
+    if (lane < 2) cp_async_4(to + (kRows + lane) * 4, lane == 0 ? w0 : w1, true);
+}
+
+// Two accumulators at once: d += v * s, element by element. Volatile: the order with the tensor memory loads around it is the
+// one that the registers were counted for.
+__device__ __forceinline__ void fma2(float2& d, uint32_t v0, uint32_t v1, float s0, float s1) {
+    asm volatile("{\n\t"
+        ".reg .b64 a, b, c;\n\t"
+        "mov.b64 a, {%2, %3};\n\t"
+        "mov.b64 b, {%4, %5};\n\t"
+        "mov.b64 c, {%0, %1};\n\t"
+        "fma.rn.f32x2 c, a, b, c;\n\t"
+        "mov.b64 {%0, %1}, c;\n\t"
+        "}"
+        : "+f"(d.x), "+f"(d.y)
+        : "r"(v0), "r"(v1), "f"(s0), "f"(s1));
+}
+
 // ---------------------------------------------------------------------------------------------------------
 // A few tokens: D[128 outputs, T tokens]
 // ---------------------------------------------------------------------------------------------------------
-constexpr int kSmallThreads = 192;   // warps 0-3 epilogue (their lane quarters of tensor memory), 4 loads, 5 multiplies
-constexpr int kScaleAhead = 4;       // k blocks that the scales are fetched ahead
-
+// T tokens per tile. Up to 64 tokens the weight is the UMMA's M side: lanes of tensor memory are outputs, columns tokens,
+// and a column's scale comes from shared memory. With T = 128 the tokens are the M side, so that a lane has one scale per
+// k block and the registers of a warp are outputs.
 template <int T>
-struct SmallSmem {
+struct SmallShape {
+    static constexpr bool kTokenLanes = T == 128;
+    static constexpr int kWidth = kTokenLanes ? 128 : T;                 // columns of an accumulator
+    static constexpr int kColumns = T == 16 ? 16 : kTokenLanes ? 64 : 32;   // ... that an epilogue warp scales
+    static constexpr int kGroups = kWidth / kColumns;
+    static constexpr int kTeams = kTokenLanes ? 1 : 2;                   // teams take the k blocks in turn
+    static constexpr int kWarps = 4 * kGroups * kTeams;
+    static constexpr int kThreads = 32 * (kWarps + 3);                   // the last three load, multiply and bring the scales
+    static constexpr int kCtasPerSm = T <= 32 ? 2 : 1;
     static constexpr int kStageBytes = kTileBytes + T * 128;
-    static constexpr int kStages = T <= 16 ? 6 : T == 32 ? 5 : T == 64 ? 4 : 3;   // two CTAs per SM
-    static constexpr int kSlots = T <= 64 ? 4 : 2;                              // accumulators in tensor memory
-    static constexpr int kScaleOff = kStages * kStageBytes;                     // [4 warps][2][T] floats
-    static constexpr int kBarOff = kScaleOff + 4 * 2 * T * 4;
+    static constexpr int kStages = T == 16 ? 6 : T == 32 ? 5 : T == 64 ? 8 : 6;
+    static constexpr int kSlots = T == 128 ? 4 : 8;                      // accumulators in tensor memory
+    static constexpr int kTmemColumns = kSlots * kWidth;
+    static constexpr int kPitch = kTokenLanes ? 132 : 128;               // floats of a token's partial sums (lanes are tokens: no bank twice)
+    static constexpr int kRaw = T + 4;                                   // floats: T token scales, the weight's, padding
+    static constexpr int kRawOff = kStages * kStageBytes;
+    static constexpr int kScaleOff = kRawOff + kScaleRing * kRaw * 4;    // [2 kSlots][T] products
+    static constexpr int kBarOff = kScaleOff + 2 * kSlots * T * 4;
     static constexpr int kNumBars = 2 * kStages + 2 * kSlots;
     static constexpr int kTotal = kBarOff + kNumBars * 8 + 16;
     static constexpr int kDynamic = kTotal + 1024;
-    static constexpr int kTmemColumns = kSlots * T < 32 ? 32 : kSlots * T;
-    static_assert(T * 512 <= kStages * kStageBytes, "the partial sums are exchanged in the operand ring");
-    static_assert(2 * (kDynamic + 1024) <= 228 * 1024 && 2 * kTmemColumns <= 512, "two CTAs per SM");
+    static_assert(kTeams * T * kPitch * 4 <= kStages * kStageBytes, "the partial sums are laid out in the operand ring");
+    static_assert(kCtasPerSm * (kDynamic + 1024) <= 228 * 1024 && kCtasPerSm * kTmemColumns <= 512, "what an SM holds");
+    static_assert(kSlots % kTeams == 0, "a team's accumulators are its own");
 };
 
 template <int T, bool kBackward, bool kOutBf16>
-__global__ void __launch_bounds__(kSmallThreads, 2) small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const Params p) {
-    using L = SmallSmem<T>;
+__global__ void __launch_bounds__(SmallShape<T>::kThreads, SmallShape<T>::kCtasPerSm)
+small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const Params p) {
+    using L = SmallShape<T>;
     extern __shared__ uint8_t smem_dyn[];
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~static_cast<uintptr_t>(1023));
     uint64_t* const full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
@@ -141,14 +196,18 @@ __global__ void __launch_bounds__(kSmallThreads, 2) small_kernel(const __grid_co
             mbar_init(&empty[s], 1);
         }
         for (int s = 0; s < L::kSlots; ++s) {
-            mbar_init(&tmem_full[s], 1);
-            mbar_init(&tmem_empty[s], 4);
+            mbar_init(&tmem_full[s], 2);
+            mbar_init(&tmem_empty[s], 4 * L::kGroups);
         }
         mbar_init_fence();
-        tma_prefetch_desc(&map_a);
-        tma_prefetch_desc(&map_w);
     }
-    if (warp == 5) {
+    if (warp == L::kWarps) {
+        if (elect_one()) {
+            tma_prefetch_desc(&map_a);
+            tma_prefetch_desc(&map_w);
+        }
+        __syncwarp();
+    } else if (warp == L::kWarps + 1) {
         tmem_alloc(tmem_slot, L::kTmemColumns);
         tmem_relinquish();
     }
@@ -163,33 +222,30 @@ __global__ void __launch_bounds__(kSmallThreads, 2) small_kernel(const __grid_co
     const int m0 = tile % p.tiles_m * T;         // row tiles fastest: the CTAs that share a weight tile run together
     const int tile_n = tile / p.tiles_m;
     const int n0 = tile_n * 128;
+    const int live = p.M - m0 < T ? p.M - m0 : T;
     const int kb_begin = static_cast<int>(static_cast<int64_t>(p.num_kb) * rank / splits);
-    const int kb_end = static_cast<int>(static_cast<int64_t>(p.num_kb) * (rank + 1) / splits);
-    const int row = warp < 4 ? warp * 32 + lane : 0;   // epilogue: output n0 + row
-    float acc[T];
+    const int blocks = static_cast<int>(static_cast<int64_t>(p.num_kb) * (rank + 1) / splits) - kb_begin;
 
-    if (warp == 4) {
+    if (warp == L::kWarps) {
+        // ---------------------------------------------------------------------- loads
         if (elect_one()) {
             grid_dependency_wait();
             Ring slot;
-            for (int kb = kb_begin; kb < kb_end; ++kb) {
+            for (int i = 0; i < blocks; ++i) {
+                const int depth0 = (kb_begin + i) * kBlock;
                 if (!guard.wait(&empty[slot.idx], slot.phase ^ 1u, kSiteLoadEmpty)) break;
                 uint8_t* const w_tile = smem + slot.idx * L::kStageBytes;
                 mbar_arrive_expect_tx(&full[slot.idx], L::kStageBytes);
-                if constexpr (kBackward) {
-                    tma_load_2d(w_tile, &map_w, &full[slot.idx], n0, kb * kBlock);
-                } else {
-                    tma_load_2d(w_tile, &map_w, &full[slot.idx], kb * kBlock, n0);
-                }
-                tma_load_2d(w_tile + kTileBytes, &map_a, &full[slot.idx], kb * kBlock, m0);
+                tma_load_2d(w_tile, &map_w, &full[slot.idx], kBackward ? n0 : depth0, kBackward ? depth0 : n0);
+                tma_load_2d(w_tile + kTileBytes, &map_a, &full[slot.idx], depth0, m0);
                 slot.advance(L::kStages);
             }
         }
-        __syncwarp();
-    } else if (warp == 5) {
+    } else if (warp == L::kWarps + 1) {
+        // ---------------------------------------------------------------------- multiplies
         if (elect_one()) {
             Ring slot, out;
-            for (int kb = kb_begin; kb < kb_end; ++kb) {
+            for (int i = 0; i < blocks; ++i) {
                 if (!guard.wait(&tmem_empty[out.idx], out.phase ^ 1u, kSiteTmemEmpty)) break;
                 if (!guard.wait(&full[slot.idx], slot.phase, kSiteLoadFull)) break;
                 tc_fence_after_sync();
@@ -198,7 +254,8 @@ __global__ void __launch_bounds__(kSmallThreads, 2) small_kernel(const __grid_co
 #pragma unroll
                 for (int k = 0; k < kBlock / 32; ++k) {
                     const uint64_t desc_w = kBackward ? make_desc_sw128_mnmajor(w_addr + k * 32 * 128) : make_desc_sw128_kmajor(w_addr + k * 32);
-                    umma_f8(tmem_base + out.idx * T, desc_w, make_desc_sw128_kmajor(a_addr + k * 32), p.idesc, k != 0 ? 1u : 0u);
+                    const uint64_t desc_a = make_desc_sw128_kmajor(a_addr + k * 32);
+                    umma_f8(tmem_base + out.idx * L::kWidth, L::kTokenLanes ? desc_a : desc_w, L::kTokenLanes ? desc_w : desc_a, p.idesc, k != 0 ? 1u : 0u);
                 }
                 umma_commit(&empty[slot.idx]);
                 umma_commit(&tmem_full[out.idx]);
@@ -206,106 +263,142 @@ __global__ void __launch_bounds__(kSmallThreads, 2) small_kernel(const __grid_co
                 out.advance(L::kSlots);
             }
         }
-        __syncwarp();
-    } else {
-        constexpr int kPerLane = (T + 31) / 32;   // token scales that a lane fetches per k block
-        float* const scales = reinterpret_cast<float*>(smem + L::kScaleOff) + warp * 2 * T;
-        float sa[kScaleAhead][kPerLane], sw[kScaleAhead];
-        const float* const w_scale = p.w_scale + tile_n * p.w_scale_out;
-        const auto fetch = [&](int kb, int at) {
-            if (kb >= kb_end) return;
-            sw[at] = __ldg(w_scale + kb * p.w_scale_block);
-#pragma unroll
-            for (int j = 0; j < kPerLane; ++j) {
-                const int token = j * 32 + lane;
-                sa[at][j] = token < T && m0 + token < p.M ? __ldg(p.a_scale + static_cast<int64_t>(kb) * p.M + m0 + token) : 0.0f;
+    } else if (warp == L::kWarps + 2) {
+        // ---------------------------------------------------------------------- scales
+        float* const raw = reinterpret_cast<float*>(smem + L::kRawOff);
+        float* const products = reinterpret_cast<float*>(smem + L::kScaleOff);
+        const float* const a_scale = p.a_scale + static_cast<int64_t>(kb_begin) * p.M + m0;
+        const float* const w_scale = p.w_scale + tile_n * p.w_scale_out + kb_begin * p.w_scale_block;
+        const auto fetch = [&](int i) {
+            if (i < blocks) {
+                const float* const w = w_scale + i * p.w_scale_block;
+                fetch_scales<T>(raw + i % kScaleRing * L::kRaw, a_scale + static_cast<int64_t>(i) * p.M, live, w, w);
             }
+            cp_async_commit();
         };
         grid_dependency_wait();
+        for (int i = 0; i < kScaleAhead; ++i) fetch(i);
+        for (int i = 0; i < blocks; ++i) {
+            cp_async_wait<kScaleAhead - 1>();
+            __syncwarp();
+            const int at = i % L::kSlots;
+            // the accumulator's previous product is complete: this arrival counts for the next one, and the scales of two
+            // products ago, which stood where these go, have been read
+            if (i >= L::kSlots && !warp_wait(guard, &tmem_full[at], static_cast<uint32_t>(i / L::kSlots - 1) & 1u, kSiteTmemFull)) break;
+            const float* const from = raw + i % kScaleRing * L::kRaw;
+            const float w = from[T];
 #pragma unroll
-        for (int t = 0; t < T; ++t) acc[t] = 0.0f;
+            for (int r = lane; r < T; r += 32) products[i % (2 * L::kSlots) * T + r] = from[r] * w;
+            fetch(i + kScaleAhead);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tmem_full[at]);
+        }
+        cp_async_wait<0>();
+    } else {
+        // ---------------------------------------------------------------------- epilogue
+        constexpr int kColumns = L::kColumns;
+        const int quarter = warp % 4;
+        const int column0 = warp / 4 % L::kGroups * kColumns;
+        const int team = warp / (4 * L::kGroups);
+        const int token = quarter * 32 + lane;   // token lanes
+        const float* const products = reinterpret_cast<const float*>(smem + L::kScaleOff);
+        const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + column0;
+        float2 acc[kColumns / 2];
 #pragma unroll
-        for (int i = 0; i < kScaleAhead; ++i) fetch(kb_begin + i, i);
-        Ring out;
+        for (int t = 0; t < kColumns / 2; ++t) acc[t] = make_float2(0.0f, 0.0f);
         bool ok = true;
-        for (int kb0 = kb_begin; ok && kb0 < kb_end; kb0 += kScaleAhead) {
+#pragma unroll 1
+        for (int i = team; i < blocks; i += L::kTeams) {
+            const int at = i % L::kSlots;
+            ok = warp_wait(guard, &tmem_full[at], static_cast<uint32_t>(i / L::kSlots) & 1u, kSiteTmemFull);
+            if (!ok) break;
+            tc_fence_after_sync();
+            const float* const scales = products + i % (2 * L::kSlots) * T;
+            if constexpr (L::kTokenLanes) {
+                uint32_t v[2][32];
+                static_assert(kColumns == 64, "two loads of 32 columns");
+                tmem_ld_32x32(taddr + at * L::kWidth, v[0]);
+                tmem_ld_32x32(taddr + at * L::kWidth + 32, v[1]);
+                const float s = scales[token];
+                tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < kScaleAhead; ++i) {
-                if (!ok || kb0 + i >= kb_end) continue;
-                float* const here = scales + (i & 1) * T;
+                for (int g = 0; g < 64; g += 2) fma2(acc[g / 2], v[g / 32][g % 32], v[g / 32][g % 32 + 1], s, s);
+            } else {
 #pragma unroll
-                for (int j = 0; j < kPerLane; ++j) {
-                    if (j * 32 + lane < T) here[j * 32 + lane] = sa[i][j] * sw[i];
-                }
-                fetch(kb0 + i + kScaleAhead, i);
-                __syncwarp();
-                ok = warp_wait(guard, &tmem_full[out.idx], out.phase, kSiteTmemFull);
-                if (!ok) continue;
-                tc_fence_after_sync();
-                const uint32_t taddr = tmem_base + (static_cast<uint32_t>(warp * 32) << 16) + out.idx * T;
-#pragma unroll
-                for (int c = 0; c < T / 16; ++c) {
+                for (int c = 0; c < kColumns; c += 16) {
                     uint32_t v[16];
-                    tmem_ld_32x16(taddr + c * 16, v);
+                    tmem_ld_32x16(taddr + at * L::kWidth + c, v);
                     tmem_wait_ld();
-                    if (c == T / 16 - 1) {
-                        tc_fence_before_sync();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&tmem_empty[out.idx]);
-                    }
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const float4 s = *reinterpret_cast<const float4*>(here + c * 16 + g * 4);
-                        acc[c * 16 + g * 4] = fmaf(__uint_as_float(v[g * 4]), s.x, acc[c * 16 + g * 4]);
-                        acc[c * 16 + g * 4 + 1] = fmaf(__uint_as_float(v[g * 4 + 1]), s.y, acc[c * 16 + g * 4 + 1]);
-                        acc[c * 16 + g * 4 + 2] = fmaf(__uint_as_float(v[g * 4 + 2]), s.z, acc[c * 16 + g * 4 + 2]);
-                        acc[c * 16 + g * 4 + 3] = fmaf(__uint_as_float(v[g * 4 + 3]), s.w, acc[c * 16 + g * 4 + 3]);
+                    for (int g = 0; g < 16; g += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(scales + column0 + c + g);
+                        fma2(acc[(c + g) / 2], v[g], v[g + 1], f.x, f.y);
+                        fma2(acc[(c + g) / 2 + 1], v[g + 2], v[g + 3], f.z, f.w);
                     }
                 }
-                out.advance(L::kSlots);
+            }
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tmem_empty[at]);
+        }
+        // Every team's sums go into this CTA's operand ring, [team][token][output]. A team may be ahead of the last block's
+        // UMMAs, which still read the ring.
+        if (ok && blocks > 0) {
+            const int last = blocks - 1;
+            (void)warp_wait(guard, &tmem_full[last % L::kSlots], static_cast<uint32_t>(last / L::kSlots) & 1u, kSiteTmemFull);
+        }
+        float* const part = reinterpret_cast<float*>(smem) + team * T * L::kPitch;
+        if constexpr (L::kTokenLanes) {
+            float4* const to = reinterpret_cast<float4*>(part + token * L::kPitch + column0);
+            if (token < live) {
+#pragma unroll
+                for (int g = 0; g < kColumns / 4; ++g) to[g] = make_float4(acc[2 * g].x, acc[2 * g].y, acc[2 * g + 1].x, acc[2 * g + 1].y);
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < kColumns; ++t) {
+                if (column0 + t < live) part[(column0 + t) * L::kPitch + quarter * 32 + lane] = t % 2 == 0 ? acc[t / 2].x : acc[t / 2].y;
             }
         }
     }
 
-    const int column = n0 + row;
-    if (splits > 1) {
-        // CTA r of the cluster owns tokens [r T / splits, ...): everybody's partial sums of them go into its operand ring
-        // ([source][token][output]), which is free in every CTA once all have met here.
-        const int share = T / splits;
-        __syncthreads();
-        cluster_sync_all();
-        if (warp < 4) {
-            const uint32_t local = smem_u32(smem) + (rank * share * 128 + row) * 4;
+    // The cluster's CTAs share the tile's tokens out and add all partial sums of theirs: split by split, team by team.
+    __syncwarp();
+    __syncthreads();
+    if (splits > 1) cluster_sync_all();
+    const int share = (live + splits - 1) / splits;
+    const int token_end = (rank + 1) * share < live ? (rank + 1) * share : live;
+    const int column = n0 + 4 * lane;
+    if (column < p.width && !guard.aborted()) {
+        float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (p.bias != nullptr) {
 #pragma unroll
-            for (int t = 0; t < T; ++t) {
-                const int owner = t / share;
-                st_shared_cluster_f32(map_to_cta(local + (t - owner * share) * 512, owner), acc[t]);
-            }
+            for (int j = 0; j < 4; ++j) bias[j] = bits_to_float<kOutBf16>(__ldg(p.bias + column + j));
         }
-        cluster_sync_all();
-        if (warp < 4 && column < p.width && !guard.aborted()) {
-            const float bias = p.bias != nullptr ? bits_to_float<kOutBf16>(__ldg(p.bias + column)) : 0.0f;
-            const float* const part = reinterpret_cast<const float*>(smem) + row;
-            for (int t = 0; t < share; ++t) {
-                const int token = m0 + rank * share + t;
-                if (token >= p.M) break;
-                float sum = part[t * 128];
-                for (int s = 1; s < splits; ++s) sum += part[(s * share + t) * 128];
-                p.c[static_cast<int64_t>(token) * p.width + column] = float_to_bits<kOutBf16>(sum + bias);
-            }
-        }
-    } else if (warp < 4 && column < p.width && !guard.aborted()) {
-        const float bias = p.bias != nullptr ? bits_to_float<kOutBf16>(__ldg(p.bias + column)) : 0.0f;
+        for (int t = rank * share + warp; t < token_end; t += L::kWarps + 3) {
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int s = 0; s < splits; ++s) {
+                const uint32_t part = map_to_cta(smem_u32(smem), static_cast<uint32_t>(s)) + (t * L::kPitch + 4 * lane) * 4;
 #pragma unroll
-        for (int t = 0; t < T; ++t) {
-            if (m0 + t < p.M) p.c[static_cast<int64_t>(m0 + t) * p.width + column] = float_to_bits<kOutBf16>(acc[t] + bias);
+                for (int team = 0; team < L::kTeams; ++team) {
+                    const float4 v = ld_shared_cluster_f32x4(part + team * T * L::kPitch * 4);
+                    sum.x += v.x;
+                    sum.y += v.y;
+                    sum.z += v.z;
+                    sum.w += v.w;
+                }
+            }
+            *reinterpret_cast<uint2*>(p.c + static_cast<int64_t>(m0 + t) * p.width + column) =
+                make_uint2(pack_out<kOutBf16>(sum.x + bias[0], sum.y + bias[1]), pack_out<kOutBf16>(sum.z + bias[2], sum.w + bias[3]));
         }
     }
 
+    __syncwarp();
     tc_fence_before_sync();
     __syncthreads();
     let_copies_land(guard);
-    if (warp == 5) {
+    if (splits > 1) cluster_sync_all();   // nobody leaves while a peer reads its sums
+    if (warp == L::kWarps + 1) {
         tc_fence_after_sync();
         tmem_dealloc(tmem_base, L::kTmemColumns);
     }
@@ -314,17 +407,24 @@ __global__ void __launch_bounds__(kSmallThreads, 2) small_kernel(const __grid_co
 // ---------------------------------------------------------------------------------------------------------
 // Many tokens: 256 tokens x tile_n outputs per CTA pair
 // ---------------------------------------------------------------------------------------------------------
+// What bounds it is the way of an accumulator from the tensor core through the epilogue's registers and back to the tensor
+// core once per 128-deep block. So a k block's product is two UMMA groups of half the tile's outputs (h = 0, 1: rows
+// h * seg .. of both CTAs' weight boxes), each with two accumulators, barriers and four epilogue warps of its own: the warps of one
+// half load accumulators from tensor memory while those of the other scale theirs.
 constexpr int kPairStages = 6;
 constexpr int kPairN = 256;
-constexpr int kPairEpilogueWarps = 8;                              // two groups of four, one per half of the outputs
-constexpr int kPairThreads = 32 * (4 + kPairEpilogueWarps);        // warps 0-3: load, multiply, relay, idle
+constexpr int kPairEpilogueWarps = 8;                              // [half][lane quarter]
+constexpr int kPairThreads = 32 * (4 + kPairEpilogueWarps);        // warps 0-3: load, multiply, relay, scales
 constexpr int kImageBytes = 32 * 64;                               // 32 rows x 32 outputs of 16 bits
 
 struct PairSmem {
     static constexpr int kStageBytes = 2 * kTileBytes;             // this CTA's 128 activation rows and its half of the outputs
-    static constexpr int kImageOff = kPairStages * kStageBytes;    // two images per epilogue warp
-    static constexpr int kBarOff = kImageOff + 2 * kPairEpilogueWarps * kImageBytes;
-    static constexpr int kNumBars = 3 * kPairStages + 4;
+    static constexpr int kImageOff = kPairStages * kStageBytes;    // one image per epilogue warp
+    static constexpr int kRaw = 132;                               // floats: 128 row scales, two of the weight's, padding
+    static constexpr int kRawOff = kImageOff + kPairEpilogueWarps * kImageBytes;
+    static constexpr int kScaleOff = kRawOff + kScaleRing * kRaw * 4;   // products [4 k blocks][2 weight blocks][128 rows]
+    static constexpr int kBarOff = kScaleOff + 4 * 2 * 128 * 4;
+    static constexpr int kNumBars = 3 * kPairStages + 8;
     static constexpr int kTotal = kBarOff + kNumBars * 8 + 16;
     static constexpr int kDynamic = kTotal + 1024;
     static_assert(kDynamic <= 227 * 1024, "the pair kernel's shared memory exceeds an SM's");
@@ -339,8 +439,8 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     uint64_t* const load_full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);   // this CTA's boxes have landed
     uint64_t* const load_empty = load_full + kPairStages;                         // signalled in both CTAs by CTA 0's commits
     uint64_t* const both_full = load_empty + kPairStages;                         // CTA 0 only: both CTAs' boxes have landed
-    uint64_t* const tmem_full = both_full + kPairStages;
-    uint64_t* const tmem_empty = tmem_full + 2;                                   // CTA 0 only
+    uint64_t* const tmem_full = both_full + kPairStages;                          // [half][accumulator]
+    uint64_t* const tmem_empty = tmem_full + 4;                                   // CTA 0 only
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(load_full + L::kNumBars);
     volatile uint32_t* const abort_flag = tmem_slot + 1;
     const int warp = static_cast<int>(threadIdx.x) / 32;
@@ -355,9 +455,9 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             mbar_init(&load_empty[s], 1);
             mbar_init(&both_full[s], 2);
         }
-        for (int s = 0; s < 2; ++s) {
-            mbar_init(&tmem_full[s], 1);
-            mbar_init(&tmem_empty[s], 2 * kPairEpilogueWarps);
+        for (int s = 0; s < 4; ++s) {
+            mbar_init(&tmem_full[s], 2);
+            mbar_init(&tmem_empty[s], kPairEpilogueWarps);   // the half's four warps of both CTAs
         }
         mbar_init_fence();
         tma_prefetch_desc(&map_a);
@@ -377,7 +477,8 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     const int num_tiles = p.tiles_m * p.tiles_n;
     const int first_tile = static_cast<int>(blockIdx.x) / 2;
     const int tile_step = static_cast<int>(gridDim.x) / 2;
-    const int half_n = p.tile_n / 2;
+    const int half_n = p.tile_n / 2;   // outputs whose weight rows (backward: columns) this CTA loads
+    const int seg = half_n / 2;        // of these, the ones in one UMMA group
 
     if (warp < 4) {
         registers_decrease<56>();
@@ -398,11 +499,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     uint8_t* const stage = smem + slot.idx * L::kStageBytes;
                     mbar_arrive_expect_tx(&load_full[slot.idx], stage_bytes);
                     tma_load_2d(stage, &map_a, &load_full[slot.idx], kb * kBlock, m0);
-                    if constexpr (kBackward) {
-                        tma_load_2d(stage + kTileBytes, &map_w, &load_full[slot.idx], n0, kb * kBlock);
-                    } else {
-                        tma_load_2d(stage + kTileBytes, &map_w, &load_full[slot.idx], kb * kBlock, n0);
-                    }
+                    tma_load_2d(stage + kTileBytes, &map_w, &load_full[slot.idx], kBackward ? n0 : kb * kBlock, kBackward ? kb * kBlock : n0);
                     slot.advance(kPairStages);
                 }
             }
@@ -412,20 +509,24 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             bool ok = true;
             for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
                 for (int kb = 0; kb < p.num_kb; ++kb) {
-                    ok = guard.wait(&tmem_empty[out.idx], out.phase ^ 1u, kSiteTmemEmpty) && guard.wait(&both_full[slot.idx], slot.phase, kSiteOperandFull);
-                    if (!ok) break;
-                    tc_fence_after_sync();
                     const uint32_t a_addr = smem_u32(smem + slot.idx * L::kStageBytes);
-                    const uint32_t w_addr = a_addr + kTileBytes;
 #pragma unroll
-                    for (int k = 0; k < kBlock / 32; ++k) {
-                        const uint64_t desc_w = kBackward ? make_desc_sw128_mnmajor(w_addr + k * 32 * 128) : make_desc_sw128_kmajor(w_addr + k * 32);
-                        umma_f8_pair(tmem_base + out.idx * kPairN, make_desc_sw128_kmajor(a_addr + k * 32), desc_w, p.idesc, k != 0 ? 1u : 0u);
+                    for (int h = 0; h < 2; ++h) {
+                        if (h == 0) ok = guard.wait(&both_full[slot.idx], slot.phase, kSiteOperandFull);
+                        ok = ok && guard.wait(&tmem_empty[2 * h + out.idx], out.phase ^ 1u, kSiteTmemEmpty);
+                        if (!ok) break;
+                        tc_fence_after_sync();
+                        // backward the weight box is MN-major: the group's outputs are bytes h * seg .. of its 128-byte rows
+                        const uint32_t w_addr = a_addr + kTileBytes + h * (kBackward ? seg : seg * 128);
+#pragma unroll
+                        for (int k = 0; k < kBlock / 32; ++k) {
+                            const uint64_t desc_w = kBackward ? make_desc_sw128_mnmajor(w_addr + k * 32 * 128) : make_desc_sw128_kmajor(w_addr + k * 32);
+                            umma_f8_pair(tmem_base + out.idx * kPairN + h * kPairN / 2, make_desc_sw128_kmajor(a_addr + k * 32), desc_w, p.idesc, k != 0 ? 1u : 0u);
+                        }
+                        umma_commit_pair_both(&tmem_full[2 * h + out.idx]);
                     }
-#pragma unroll
-                    for (uint32_t dst = 0; dst < 2; ++dst) umma_commit_pair(map_to_cta(smem_u32(&load_empty[slot.idx]), dst));
-#pragma unroll
-                    for (uint32_t dst = 0; dst < 2; ++dst) umma_commit_pair(map_to_cta(smem_u32(&tmem_full[out.idx]), dst));
+                    if (!ok) break;
+                    umma_commit_pair_both(&load_empty[slot.idx]);
                     slot.advance(kPairStages);
                     out.advance(2);
                 }
@@ -442,93 +543,144 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     slot.advance(kPairStages);
                 }
             }
+        } else if (warp == 3) {
+            // ------------------------------------------------------------------ scales of this CTA's rows
+            float* const raw = reinterpret_cast<float*>(smem + L::kRawOff);
+            float* const products = reinterpret_cast<float*>(smem + L::kScaleOff);
+            // the block that is fetched next, kScaleAhead blocks before the one that is multiplied: it may be of the next tile
+            int tile = first_tile, kb = 0, live = 0;
+            const float *a_scale = p.a_scale, *w0 = p.w_scale, *w1 = p.w_scale;
+            const auto enter = [&]() {
+                if (tile >= num_tiles) return;
+                int tile_m, tile_n;
+                banded_tile(tile, p.tiles_m, p.tiles_n, p.band, tile_m, tile_n);
+                const int row0 = tile_m * 256 + static_cast<int>(cta) * 128, col0 = tile_n * p.tile_n;
+                live = p.M - row0;
+                a_scale = p.a_scale + (live > 0 ? row0 : 0);
+                // half_n divides 128: the outputs of a CTA's weight rows have one block of weight scales
+                w0 = p.w_scale + col0 / kBlock * p.w_scale_out;
+                w1 = col0 + half_n < p.width ? p.w_scale + (col0 + half_n) / kBlock * p.w_scale_out : w0;
+            };
+            const auto fetch = [&](uint32_t turn) {
+                if (tile < num_tiles) {
+                    fetch_scales<128>(raw + turn % kScaleRing * L::kRaw, a_scale, live, w0, w1);
+                    a_scale += p.M;
+                    w0 += p.w_scale_block;
+                    w1 += p.w_scale_block;
+                    if (++kb == p.num_kb) {
+                        kb = 0;
+                        tile += tile_step;
+                        enter();
+                    }
+                }
+                cp_async_commit();
+            };
+            grid_dependency_wait();
+            enter();
+            for (uint32_t i = 0; i < kScaleAhead; ++i) fetch(i);
+            const uint32_t turns = first_tile < num_tiles ? static_cast<uint32_t>((num_tiles - 1 - first_tile) / tile_step + 1) * static_cast<uint32_t>(p.num_kb) : 0u;
+            for (uint32_t turn = 0; turn < turns; ++turn) {
+                cp_async_wait<kScaleAhead - 1>();
+                __syncwarp();
+                const uint32_t slot = turn & 1u;
+                // the accumulators' previous products are complete: this arrival counts for the next ones, and the scales of four
+                // blocks ago, which stood where these go, have been read
+                if (turn >= 2 && !(warp_wait(guard, &tmem_full[slot], ((turn >> 1) - 1) & 1u, kSiteTmemFull) &&
+                                   warp_wait(guard, &tmem_full[2 + slot], ((turn >> 1) - 1) & 1u, kSiteTmemFull))) {
+                    break;
+                }
+                const float* const from = raw + turn % kScaleRing * L::kRaw;
+                float* const to = products + (turn & 3u) * 256;
+                const float s0 = from[128], s1 = from[129];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float sa = from[r * 32 + lane];
+                    to[r * 32 + lane] = sa * s0;
+                    to[128 + r * 32 + lane] = sa * s1;
+                }
+                fetch(turn + kScaleAhead);
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&tmem_full[slot]);
+                    mbar_arrive(&tmem_full[2 + slot]);
+                }
+            }
+            cp_async_wait<0>();
         }
     } else {
         registers_increase<216>();
-        // ---------------------------------------------------------------------- epilogue: this CTA's 128 rows, half of the outputs per group
-        const int epi_warp = warp - 4;
+        // ---------------------------------------------------------------------- epilogue: this CTA's 128 rows
         const int quarter = warp % 4;
-        const int half = epi_warp / 4;
-        const int chunks = half_n / 32;
+        const int half = (warp - 4) / 4;
+        const int chunks = 2 * seg / 32;     // of 32 outputs: those of CTA 0's weight rows, then CTA 1's
         const int twist = (lane >> 1) & 3;   // 64-byte swizzle: the 16-byte chunk index is XORed with bits 7-8 of the address
-        uint8_t* const images = smem + L::kImageOff + epi_warp * 2 * kImageBytes;
-        uint32_t stores = 0;
-        Ring out;
+        uint8_t* const image = smem + L::kImageOff + (warp - 4) * kImageBytes;
+        const float* const products = reinterpret_cast<const float*>(smem + L::kScaleOff) + quarter * 32 + lane;
+        const uint32_t empty0 = map_to_cta(smem_u32(tmem_empty + 2 * half), 0);
+        const uint32_t taddr0 = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + half * (kPairN / 2);
+        bool stored = false;
+        uint32_t turn = 0;   // k blocks so far: their accumulators alternate
         bool ok = true;
-        grid_dependency_wait();
+        grid_dependency_wait();   // the kernel before this one may still read what this one writes
         for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
             int tile_m, tile_n;
             banded_tile(tile, p.tiles_m, p.tiles_n, p.band, tile_m, tile_n);
             const int row0 = tile_m * 256 + static_cast<int>(cta) * 128 + quarter * 32;
-            const int col0 = tile_n * p.tile_n + half * half_n;
-            // half_n is a multiple of 32 and at most 128: the columns meet at most two blocks of the weight's scales, and the
-            // border lies between two chunks
-            const int block_lo = col0 / kBlock;
-            const int border = ((block_lo + 1) * kBlock - col0) / 32;   // first chunk of the second block
-            const bool two = border < chunks && (block_lo + 1) * kBlock < p.width;
-            const float* const a_scale = p.a_scale + (row0 + lane < p.M ? row0 + lane : 0);
-            const float* const w_lo = p.w_scale + (col0 < p.width ? block_lo : 0) * p.w_scale_out;
-            const float* const w_hi = two ? w_lo + p.w_scale_out : w_lo;
-            float acc[128];
+            const int col0 = tile_n * p.tile_n;
+            float2 acc[4][16];
 #pragma unroll
-            for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
-            float sa[kScaleAhead], lo[kScaleAhead], hi[kScaleAhead];
-            const auto fetch = [&](int kb, int at) {
-                if (kb >= p.num_kb) return;
-                sa[at] = __ldg(a_scale + static_cast<int64_t>(kb) * p.M);
-                lo[at] = __ldg(w_lo + kb * p.w_scale_block);
-                hi[at] = __ldg(w_hi + kb * p.w_scale_block);
-            };
+            for (int i = 0; i < 64; ++i) acc[i / 16][i % 16] = make_float2(0.0f, 0.0f);
+#pragma unroll 1
+            for (int kb = 0; kb < p.num_kb; ++kb, ++turn) {
+                const uint32_t slot = turn & 1u;
+                ok = warp_wait(guard, &tmem_full[2 * half + slot], (turn >> 1) & 1u, kSiteTmemFull);
+                if (!ok) break;
+                tc_fence_after_sync();
+                const uint32_t taddr = taddr0 + slot * kPairN;
+                uint32_t v[2][32];
+                tmem_ld_32x32(taddr, v[0]);
+                const float s0 = products[(turn & 3u) * 256], s1 = products[(turn & 3u) * 256 + 128];
+                tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < kScaleAhead; ++i) fetch(i, i);
-            for (int kb0 = 0; ok && kb0 < p.num_kb; kb0 += kScaleAhead) {
+                for (int c = 0; c < 4; ++c) {
+                    if (c < chunks) {
+                        if (c + 1 < chunks) tmem_ld_32x32(taddr + (c + 1) % 4 * 32, v[(c + 1) % 2]);
+                        const float s = 2 * c < chunks ? s0 : s1;
 #pragma unroll
-                for (int i = 0; i < kScaleAhead; ++i) {
-                    if (!ok || kb0 + i >= p.num_kb) continue;
-                    const float s_lo = sa[i] * lo[i], s_hi = sa[i] * hi[i];
-                    fetch(kb0 + i + kScaleAhead, i);
-                    ok = warp_wait(guard, &tmem_full[out.idx], out.phase, kSiteTmemFull);
-                    if (!ok) continue;
-                    tc_fence_after_sync();
-                    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + out.idx * kPairN + half * half_n;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        if (c < chunks) {
-                            uint32_t v[32];
-                            tmem_ld_32x32(taddr + c * 32, v);
-                            tmem_wait_ld();
-                            const float s = c < border ? s_lo : s_hi;
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) acc[c * 32 + j] = fmaf(__uint_as_float(v[j]), s, acc[c * 32 + j]);
+                        for (int j = 0; j < 16; ++j) fma2(acc[c][j], v[c % 2][2 * j], v[c % 2][2 * j + 1], s, s);
+                        if (c + 1 < chunks) tmem_wait_ld();
+                        if (c + 2 == chunks) {
+                            tc_fence_before_sync();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive_cluster(empty0 + slot * 8);
                         }
                     }
-                    tc_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&tmem_empty[out.idx]), 0));
-                    out.advance(2);
                 }
             }
             if (!ok) break;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const int column = col0 + c * 32;
+                const bool other = 2 * c >= chunks;   // CTA 1's weight rows
+                const int column = col0 + half * seg + (other ? half_n + (c - chunks / 2) * 32 : c * 32);
                 if (c >= chunks || column >= p.width || row0 >= p.M) continue;
                 if (p.bias != nullptr) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        if (column + j < p.width) acc[c * 32 + j] += bits_to_float<kOutBf16>(__ldg(p.bias + column + j));
+                    for (int j = 0; j < 16; ++j) {
+                        if (column + 2 * j < p.width) {
+                            acc[c][j].x += bits_to_float<kOutBf16>(__ldg(p.bias + column + 2 * j));
+                            acc[c][j].y += bits_to_float<kOutBf16>(__ldg(p.bias + column + 2 * j + 1));
+                        }
                     }
                 }
-                if (stores >= 2) {   // the image's earlier store has been read
-                    if (lane == 0) tma_store_wait_read<1>();
+                if (stored) {   // the image's earlier store has been read
+                    if (lane == 0) tma_store_wait_read<0>();
                     __syncwarp();
                 }
-                uint8_t* const image = images + (stores & 1u) * kImageBytes;
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const float* const v = acc + c * 32 + g * 8;
+                    const float2* const f = acc[c] + g * 4;
                     *reinterpret_cast<uint4*>(image + lane * 64 + ((g ^ twist) << 4)) =
-                        make_uint4(pack_out<kOutBf16>(v[0], v[1]), pack_out<kOutBf16>(v[2], v[3]), pack_out<kOutBf16>(v[4], v[5]), pack_out<kOutBf16>(v[6], v[7]));
+                        make_uint4(pack_out<kOutBf16>(f[0].x, f[0].y), pack_out<kOutBf16>(f[1].x, f[1].y), pack_out<kOutBf16>(f[2].x, f[2].y), pack_out<kOutBf16>(f[3].x, f[3].y));
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -536,7 +688,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     tma_store_2d(&map_c, image, column, row0);   // clipped at M and width
                     tma_store_commit();
                 }
-                ++stores;
+                stored = true;
             }
         }
         if (lane == 0) tma_store_wait<0>();
@@ -604,7 +756,7 @@ uint32_t format(bool e5m2) { return e5m2 ? kFmtE5M2 : kFmtE4M3; }
 
 template <int T, bool kBackward, bool kOutBf16>
 bool launch_small_instance(const Args& args, int splits) {
-    using L = SmallSmem<T>;
+    using L = SmallShape<T>;
     auto* const kernel = &small_kernel<T, kBackward, kOutBf16>;
     static PerDeviceState ready;
     if (ready.get([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDynamic) == cudaSuccess ? 1 : 0; }) <= 0) return false;
@@ -616,10 +768,11 @@ bool launch_small_instance(const Args& args, int splits) {
     p.tiles_m = static_cast<int>(tiles_m);
     p.tiles_n = static_cast<int>(tiles_n);
     p.splits = splits;
-    p.idesc = make_idesc(kAccF32, format(args.w_e5m2), format(args.a_e5m2), 128, T) | (kBackward ? kIdescAMajorMN : 0u);
+    p.idesc = L::kTokenLanes ? make_idesc(kAccF32, format(args.a_e5m2), format(args.w_e5m2), 128, 128) | (kBackward ? kIdescBMajorMN : 0u)
+                             : make_idesc(kAccF32, format(args.w_e5m2), format(args.a_e5m2), 128, T) | (kBackward ? kIdescAMajorMN : 0u);
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(static_cast<unsigned>(tiles_m * tiles_n * splits));
-    config.blockDim = dim3(kSmallThreads);
+    config.blockDim = dim3(L::kThreads);
     config.dynamicSmemBytes = L::kDynamic;
     config.stream = args.stream;
     cudaLaunchAttribute attr[2];
@@ -685,7 +838,7 @@ bool launch_pair(const Args& args, int tile_n) {
     int64_t band = (32ll << 20) / (256 * args.depth());   // about 32 MB of activations stay in L2 while a band sweeps the weight
     if (band < 4) band = 4;
     p.band = static_cast<int>(band < tiles_m ? band : tiles_m);
-    p.idesc = make_idesc(kAccF32, format(args.a_e5m2), format(args.w_e5m2), 256, static_cast<uint32_t>(tile_n)) | (kBackward ? kIdescBMajorMN : 0u);
+    p.idesc = make_idesc(kAccF32, format(args.a_e5m2), format(args.w_e5m2), 256, static_cast<uint32_t>(tile_n / 2)) | (kBackward ? kIdescBMajorMN : 0u);
     cudaLaunchConfig_t config = {};
     const int64_t tiles = tiles_m * tiles_n;
     config.gridDim = dim3(static_cast<unsigned>(2 * (tiles < pairs ? tiles : pairs)));
@@ -703,7 +856,7 @@ bool launch_pair(const Args& args, int tile_n) {
 // Which kernel a product gets.
 struct Plan {
     int tokens;   // small kernel: tokens per tile; 0: pair kernel
-    int splits;   // small kernel: K splits (1, 2, 4 or 8)
+    int splits;   // small kernel: K splits, at most 8
     int tile_n;   // pair kernel: outputs per tile
 };
 

@@ -316,8 +316,11 @@ __device__ __forceinline__ void st_shared_cluster_v4(uint32_t cluster_addr, uint
     asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
-__device__ __forceinline__ void st_shared_cluster_f32(uint32_t cluster_addr, float v) {
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
+// 16 bytes from a CTA's shared memory (this one's or a peer's)
+__device__ __forceinline__ float4 ld_shared_cluster_f32x4(uint32_t cluster_addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr) : "memory");
+    return v;
 }
 
 // Arrive on a barrier given by its shared::cluster address (this CTA's or the peer's). Plain release
@@ -342,6 +345,11 @@ __device__ __forceinline__ void tmem_dealloc_pair(uint32_t base, uint32_t column
 // arrive (once the pair's UMMAs issued so far have completed) on the barrier at `cluster_addr`
 __device__ __forceinline__ void umma_commit_pair(uint32_t cluster_addr) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// ... on the barrier at `bar`'s place in both CTAs of the pair (a commit is not a load: nothing of memory is multicast)
+__device__ __forceinline__ void umma_commit_pair_both(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"(static_cast<uint16_t>(3)) : "memory");
 }
 
 __device__ __forceinline__ void umma_f16_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
