@@ -9,10 +9,10 @@
 // and backward, where the contraction runs over the weight's rows, the same box is an MN-major operand.
 //
 // Two kernels, picked by `plan`:
-//   * small_kernel: the weight is the M side of the UMMA (128 outputs per CTA) and 16 to 128 tokens its N side, so a few
-//     tokens cost no padding to 128 rows. K is split over the CTAs of a cluster, which add their partial sums through
+//   * small_kernel: 128 outputs x 16, 32 or 128 tokens per CTA; for up to 32 tokens the weight is the M side of the UMMA,
+//     so that a few tokens cost no padding to 128 rows. K is split over the CTAs of a cluster, which add their partial sums through
 //     distributed shared memory in a fixed order.
-//   * pair_kernel: 256 tokens x up to 256 outputs per CTA pair, persistent.
+//   * pair_kernel: 256 tokens x 256 outputs per CTA pair, persistent.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -27,6 +27,7 @@ namespace f8mm {
 
 constexpr int kBlock = 128;          // depth of a k block = channels per scale
 constexpr int kTileBytes = 128 * 128;
+constexpr int kMaxSplits = 8;        // CTAs of a cluster along the contraction (the largest portable cluster)
 
 __device__ uint32_t g_status[2];
 
@@ -40,7 +41,7 @@ struct Params {
     int M, width, num_kb;
     int tiles_m, tiles_n;
     int splits;              // small kernel: CTAs of a cluster along the contraction
-    int tile_n, band;        // pair kernel: outputs per tile, row tiles per band of the walk
+    int band;                // pair kernel: row tiles per band of the walk
     uint32_t idesc;
 };
 
@@ -143,38 +144,40 @@ __device__ __forceinline__ void fma2(float2& d, uint32_t v0, uint32_t v1, float 
 // ---------------------------------------------------------------------------------------------------------
 // A few tokens: D[128 outputs, T tokens]
 // ---------------------------------------------------------------------------------------------------------
-// T tokens per tile. Up to 64 tokens the weight is the UMMA's M side: lanes of tensor memory are outputs, columns tokens,
+// T tokens per tile. Up to 32 tokens the weight is the UMMA's M side: lanes of tensor memory are outputs, columns tokens,
 // and a column's scale comes from shared memory. With T = 128 the tokens are the M side, so that a lane has one scale per
-// k block and the registers of a warp are outputs.
+// k block and the registers of a warp are outputs. (64 tokens as columns were never faster than 128 lanes: 64 x 5120 x 5120
+// in three K splits 13.0 us against 10.9.)
 template <int T>
 struct SmallShape {
     static constexpr bool kTokenLanes = T == 128;
     static constexpr int kWidth = kTokenLanes ? 128 : T;                 // columns of an accumulator
-    static constexpr int kColumns = T == 16 ? 16 : kTokenLanes ? 64 : 32;   // ... that an epilogue warp scales
+    static constexpr int kColumns = kTokenLanes ? 64 : T;                // ... that an epilogue warp scales
     static constexpr int kGroups = kWidth / kColumns;
     static constexpr int kTeams = kTokenLanes ? 1 : 2;                   // teams take the k blocks in turn
     static constexpr int kWarps = 4 * kGroups * kTeams;
     static constexpr int kThreads = 32 * (kWarps + 3);                   // the last three load, multiply and bring the scales
-    static constexpr int kCtasPerSm = T <= 32 ? 2 : 1;
     static constexpr int kStageBytes = kTileBytes + T * 128;
-    static constexpr int kStages = T == 16 ? 6 : T == 32 ? 5 : T == 64 ? 8 : 6;
+    static constexpr int kStages = T == 16 ? 11 : T == 32 ? 10 : 6;
     static constexpr int kSlots = T == 128 ? 4 : 8;                      // accumulators in tensor memory
     static constexpr int kTmemColumns = kSlots * kWidth;
     static constexpr int kPitch = kTokenLanes ? 132 : 128;               // floats of a token's partial sums (lanes are tokens: no bank twice)
     static constexpr int kRaw = T + 4;                                   // floats: T token scales, the weight's, padding
     static constexpr int kRawOff = kStages * kStageBytes;
-    static constexpr int kScaleOff = kRawOff + kScaleRing * kRaw * 4;    // [2 kSlots][T] products
+    static constexpr int kBatch = kSlots / 2;                            // k blocks that the scale warp does at a time
+    static constexpr int kRawRing = 4 * kBatch;                          // fetched two batches ahead
+    static constexpr int kScaleOff = kRawOff + kRawRing * kRaw * 4;      // [2 kSlots][T] products
     static constexpr int kBarOff = kScaleOff + 2 * kSlots * T * 4;
     static constexpr int kNumBars = 2 * kStages + 2 * kSlots;
     static constexpr int kTotal = kBarOff + kNumBars * 8 + 16;
     static constexpr int kDynamic = kTotal + 1024;
     static_assert(kTeams * T * kPitch * 4 <= kStages * kStageBytes, "the partial sums are laid out in the operand ring");
-    static_assert(kCtasPerSm * (kDynamic + 1024) <= 228 * 1024 && kCtasPerSm * kTmemColumns <= 512, "what an SM holds");
+    static_assert(kDynamic <= 227 * 1024 && kTmemColumns <= 512, "what an SM holds");
     static_assert(kSlots % kTeams == 0, "a team's accumulators are its own");
 };
 
 template <int T, bool kBackward, bool kOutBf16>
-__global__ void __launch_bounds__(SmallShape<T>::kThreads, SmallShape<T>::kCtasPerSm)
+__global__ void __launch_bounds__(SmallShape<T>::kThreads, 1)
 small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const Params p) {
     using L = SmallShape<T>;
     extern __shared__ uint8_t smem_dyn[];
@@ -264,34 +267,43 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
             }
         }
     } else if (warp == L::kWarps + 2) {
-        // ---------------------------------------------------------------------- scales
+        // ---------------------------------------------------------------------- scales, kBatch k blocks at a time
+        constexpr int kBatch = L::kBatch;
         float* const raw = reinterpret_cast<float*>(smem + L::kRawOff);
         float* const products = reinterpret_cast<float*>(smem + L::kScaleOff);
-        const float* const a_scale = p.a_scale + static_cast<int64_t>(kb_begin) * p.M + m0;
-        const float* const w_scale = p.w_scale + tile_n * p.w_scale_out + kb_begin * p.w_scale_block;
-        const auto fetch = [&](int i) {
-            if (i < blocks) {
-                const float* const w = w_scale + i * p.w_scale_block;
-                fetch_scales<T>(raw + i % kScaleRing * L::kRaw, a_scale + static_cast<int64_t>(i) * p.M, live, w, w);
+        const float* a_scale = p.a_scale + static_cast<int64_t>(kb_begin) * p.M + m0;
+        const float* w_scale = p.w_scale + tile_n * p.w_scale_out + kb_begin * p.w_scale_block;
+        const auto fetch = [&](int i0) {
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) {
+                if (i0 + j < blocks) {
+                    fetch_scales<T>(raw + (i0 + j) % L::kRawRing * L::kRaw, a_scale, live, w_scale, w_scale);
+                    a_scale += p.M;
+                    w_scale += p.w_scale_block;
+                }
             }
             cp_async_commit();
         };
         grid_dependency_wait();
-        for (int i = 0; i < kScaleAhead; ++i) fetch(i);
-        for (int i = 0; i < blocks; ++i) {
-            cp_async_wait<kScaleAhead - 1>();
+        fetch(0);
+        fetch(kBatch);
+        for (int i0 = 0; i0 < blocks; i0 += kBatch) {
+            cp_async_wait<1>();
             __syncwarp();
-            const int at = i % L::kSlots;
-            // the accumulator's previous product is complete: this arrival counts for the next one, and the scales of two
-            // products ago, which stood where these go, have been read
-            if (i >= L::kSlots && !warp_wait(guard, &tmem_full[at], static_cast<uint32_t>(i / L::kSlots - 1) & 1u, kSiteTmemFull)) break;
-            const float* const from = raw + i % kScaleRing * L::kRaw;
-            const float w = from[T];
+            // The accumulators' previous products are complete (they come in order, so the last one's is enough): these arrivals
+            // count for the next ones, and the scales of two products ago, which stood where these go, have been read.
+            const int before = i0 + kBatch - 1 - L::kSlots;
+            if (before >= 0 && !warp_wait(guard, &tmem_full[before % L::kSlots], static_cast<uint32_t>(before / L::kSlots) & 1u, kSiteTmemFull)) break;
 #pragma unroll
-            for (int r = lane; r < T; r += 32) products[i % (2 * L::kSlots) * T + r] = from[r] * w;
-            fetch(i + kScaleAhead);
+            for (int j = 0; j < kBatch; ++j) {
+                const float* const from = raw + (i0 + j) % L::kRawRing * L::kRaw;
+                const float w = from[T];   // of blocks past the end: whatever stands there, nobody reads the products
+#pragma unroll
+                for (int r = lane; r < T; r += 32) products[(i0 + j) % (2 * L::kSlots) * T + r] = from[r] * w;
+            }
+            fetch(i0 + 2 * kBatch);
             __syncwarp();
-            if (lane == 0) mbar_arrive(&tmem_full[at]);
+            if (lane < kBatch && i0 + lane < blocks) mbar_arrive(&tmem_full[(i0 + lane) % L::kSlots]);
         }
         cp_async_wait<0>();
     } else {
@@ -405,7 +417,7 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// Many tokens: 256 tokens x tile_n outputs per CTA pair
+// Many tokens: 256 tokens x 256 outputs per CTA pair
 // ---------------------------------------------------------------------------------------------------------
 // What bounds it is the way of an accumulator from the tensor core through the epilogue's registers and back to the tensor
 // core once per 128-deep block. So a k block's product is two UMMA groups of half the tile's outputs (h = 0, 1: rows
@@ -477,8 +489,8 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     const int num_tiles = p.tiles_m * p.tiles_n;
     const int first_tile = static_cast<int>(blockIdx.x) / 2;
     const int tile_step = static_cast<int>(gridDim.x) / 2;
-    const int half_n = p.tile_n / 2;   // outputs whose weight rows (backward: columns) this CTA loads
-    const int seg = half_n / 2;        // of these, the ones in one UMMA group
+    constexpr int half_n = kPairN / 2;   // outputs whose weight rows (backward: columns) this CTA loads
+    constexpr int seg = half_n / 2;      // of these, the ones in one UMMA group
 
     if (warp < 4) {
         registers_decrease<56>();
@@ -492,7 +504,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 int tile_m, tile_n;
                 banded_tile(tile, p.tiles_m, p.tiles_n, p.band, tile_m, tile_n);
                 const int m0 = tile_m * 256 + static_cast<int>(cta) * 128;
-                const int n0 = tile_n * p.tile_n + static_cast<int>(cta) * half_n;
+                const int n0 = tile_n * kPairN + static_cast<int>(cta) * half_n;
                 for (int kb = 0; kb < p.num_kb; ++kb) {
                     ok = guard.wait(&load_empty[slot.idx], slot.phase ^ 1u, kSiteLoadEmpty);
                     if (!ok) break;
@@ -554,10 +566,10 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 if (tile >= num_tiles) return;
                 int tile_m, tile_n;
                 banded_tile(tile, p.tiles_m, p.tiles_n, p.band, tile_m, tile_n);
-                const int row0 = tile_m * 256 + static_cast<int>(cta) * 128, col0 = tile_n * p.tile_n;
+                const int row0 = tile_m * 256 + static_cast<int>(cta) * 128, col0 = tile_n * kPairN;
                 live = p.M - row0;
                 a_scale = p.a_scale + (live > 0 ? row0 : 0);
-                // half_n divides 128: the outputs of a CTA's weight rows have one block of weight scales
+                // half_n is a block: the outputs of a CTA's weight rows have one block of weight scales
                 w0 = p.w_scale + col0 / kBlock * p.w_scale_out;
                 w1 = col0 + half_n < p.width ? p.w_scale + (col0 + half_n) / kBlock * p.w_scale_out : w0;
             };
@@ -612,7 +624,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         // ---------------------------------------------------------------------- epilogue: this CTA's 128 rows
         const int quarter = warp % 4;
         const int half = (warp - 4) / 4;
-        const int chunks = 2 * seg / 32;     // of 32 outputs: those of CTA 0's weight rows, then CTA 1's
+        constexpr int kChunks = 2 * seg / 32;   // of 32 outputs: those of CTA 0's weight rows, then CTA 1's
         const int twist = (lane >> 1) & 3;   // 64-byte swizzle: the 16-byte chunk index is XORed with bits 7-8 of the address
         uint8_t* const image = smem + L::kImageOff + (warp - 4) * kImageBytes;
         const float* const products = reinterpret_cast<const float*>(smem + L::kScaleOff) + quarter * 32 + lane;
@@ -626,43 +638,50 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             int tile_m, tile_n;
             banded_tile(tile, p.tiles_m, p.tiles_n, p.band, tile_m, tile_n);
             const int row0 = tile_m * 256 + static_cast<int>(cta) * 128 + quarter * 32;
-            const int col0 = tile_n * p.tile_n;
-            float2 acc[4][16];
+            const int col0 = tile_n * kPairN;
+            float2 acc[kChunks][16];
 #pragma unroll
-            for (int i = 0; i < 64; ++i) acc[i / 16][i % 16] = make_float2(0.0f, 0.0f);
+            for (int i = 0; i < 16 * kChunks; ++i) acc[i / 16][i % 16] = make_float2(0.0f, 0.0f);
+            // Four chunks of 32 columns per k block, one being loaded while the one before is scaled, across
+            // k blocks too: the last chunk of a block is scaled while the first of the next one comes.
+            uint32_t v[2][32];
+            ok = warp_wait(guard, &tmem_full[2 * half + (turn & 1u)], (turn >> 1) & 1u, kSiteTmemFull);
+            if (!ok) break;
+            tc_fence_after_sync();
+            tmem_ld_32x32(taddr0 + (turn & 1u) * kPairN, v[0]);
 #pragma unroll 1
-            for (int kb = 0; kb < p.num_kb; ++kb, ++turn) {
+            for (int kb = 0; kb < p.num_kb; ++kb) {
                 const uint32_t slot = turn & 1u;
-                ok = warp_wait(guard, &tmem_full[2 * half + slot], (turn >> 1) & 1u, kSiteTmemFull);
-                if (!ok) break;
-                tc_fence_after_sync();
                 const uint32_t taddr = taddr0 + slot * kPairN;
-                uint32_t v[2][32];
-                tmem_ld_32x32(taddr, v[0]);
                 const float s0 = products[(turn & 3u) * 256], s1 = products[(turn & 3u) * 256 + 128];
-                tmem_wait_ld();
+                ++turn;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    if (c < chunks) {
-                        if (c + 1 < chunks) tmem_ld_32x32(taddr + (c + 1) % 4 * 32, v[(c + 1) % 2]);
-                        const float s = 2 * c < chunks ? s0 : s1;
+                for (int c = 0; c < 3; ++c) {
+                    tmem_wait_ld();
+                    tmem_ld_32x32(taddr + (c + 1) * 32, v[(c + 1) % 2]);
+                    const float s = 2 * c < kChunks ? s0 : s1;
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) fma2(acc[c][j], v[c % 2][2 * j], v[c % 2][2 * j + 1], s, s);
-                        if (c + 1 < chunks) tmem_wait_ld();
-                        if (c + 2 == chunks) {
-                            tc_fence_before_sync();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive_cluster(empty0 + slot * 8);
-                        }
-                    }
+                    for (int j = 0; j < 16; ++j) fma2(acc[c][j], v[c % 2][2 * j], v[c % 2][2 * j + 1], s, s);
                 }
+                tmem_wait_ld();
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(empty0 + slot * 8);
+                if (kb + 1 < p.num_kb) {
+                    ok = warp_wait(guard, &tmem_full[2 * half + (turn & 1u)], (turn >> 1) & 1u, kSiteTmemFull);
+                    if (!ok) break;
+                    tc_fence_after_sync();
+                    tmem_ld_32x32(taddr0 + (turn & 1u) * kPairN, v[0]);
+                }
+#pragma unroll
+                for (int j = 0; j < 16; ++j) fma2(acc[kChunks - 1][j], v[1][2 * j], v[1][2 * j + 1], s1, s1);
             }
             if (!ok) break;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const bool other = 2 * c >= chunks;   // CTA 1's weight rows
-                const int column = col0 + half * seg + (other ? half_n + (c - chunks / 2) * 32 : c * 32);
-                if (c >= chunks || column >= p.width || row0 >= p.M) continue;
+            for (int c = 0; c < kChunks; ++c) {
+                const bool other = 2 * c >= kChunks;   // CTA 1's weight rows
+                const int column = col0 + half * seg + (other ? half_n + (c - kChunks / 2) * 32 : c * 32);
+                if (column >= p.width || row0 >= p.M) continue;
                 if (p.bias != nullptr) {
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
@@ -755,11 +774,43 @@ bool make_maps(const Args& args, int a_rows, int w_rows, CUtensorMap& map_a, CUt
 uint32_t format(bool e5m2) { return e5m2 ? kFmtE5M2 : kFmtE4M3; }
 
 template <int T, bool kBackward, bool kOutBf16>
-bool launch_small_instance(const Args& args, int splits) {
+cudaLaunchConfig_t small_config(cudaLaunchAttribute* attr, int64_t grid, int splits) {
     using L = SmallShape<T>;
-    auto* const kernel = &small_kernel<T, kBackward, kOutBf16>;
-    static PerDeviceState ready;
-    if (ready.get([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDynamic) == cudaSuccess ? 1 : 0; }) <= 0) return false;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(static_cast<unsigned>(grid));
+    config.blockDim = dim3(L::kThreads);
+    config.dynamicSmemBytes = L::kDynamic;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(splits);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    config.attrs = attr;
+    config.numAttrs = 1;
+    return config;
+}
+
+// How many clusters of `splits` CTAs the device holds at once (0: none, or the kernel cannot be prepared). Asked once per
+// device: clusters live within a GPC, so 148 SMs hold 45 clusters of three and 15 of eight.
+template <int T, bool kBackward, bool kOutBf16>
+int small_clusters(int splits) {
+    static PerDeviceState resident[kMaxSplits + 1];
+    return resident[splits].get([&] {
+        auto* const kernel = &small_kernel<T, kBackward, kOutBf16>;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SmallShape<T>::kDynamic) != cudaSuccess) return 0;
+        cudaLaunchAttribute attr[2];
+        const cudaLaunchConfig_t config = small_config<T, kBackward, kOutBf16>(attr, device_info().sm_count / splits * splits, splits);
+        int clusters = 0;
+        if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &config) != cudaSuccess) {
+            (void)cudaGetLastError();
+            clusters = 0;
+        }
+        return clusters;
+    });
+}
+
+template <int T, bool kBackward, bool kOutBf16>
+bool launch_small(const Args& args, int splits) {
+    if (small_clusters<T, kBackward, kOutBf16>(splits) <= 0) return false;
     CUtensorMap map_a, map_w;
     if (!make_maps(args, T, 128, map_a, map_w)) return false;
     Params p = make_params(args);
@@ -768,37 +819,19 @@ bool launch_small_instance(const Args& args, int splits) {
     p.tiles_m = static_cast<int>(tiles_m);
     p.tiles_n = static_cast<int>(tiles_n);
     p.splits = splits;
-    p.idesc = L::kTokenLanes ? make_idesc(kAccF32, format(args.a_e5m2), format(args.w_e5m2), 128, 128) | (kBackward ? kIdescBMajorMN : 0u)
-                             : make_idesc(kAccF32, format(args.w_e5m2), format(args.a_e5m2), 128, T) | (kBackward ? kIdescAMajorMN : 0u);
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(static_cast<unsigned>(tiles_m * tiles_n * splits));
-    config.blockDim = dim3(L::kThreads);
-    config.dynamicSmemBytes = L::kDynamic;
-    config.stream = args.stream;
+    p.idesc = SmallShape<T>::kTokenLanes ? make_idesc(kAccF32, format(args.a_e5m2), format(args.w_e5m2), 128, 128) | (kBackward ? kIdescBMajorMN : 0u)
+                                         : make_idesc(kAccF32, format(args.w_e5m2), format(args.a_e5m2), 128, T) | (kBackward ? kIdescAMajorMN : 0u);
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(splits);
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t config = small_config<T, kBackward, kOutBf16>(attr, tiles_m * tiles_n * splits, splits);
+    config.stream = args.stream;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = attr;
-    config.numAttrs = args.after_quantizer ? 2 : 1;
-    return cudaLaunchKernelEx(&config, kernel, map_a, map_w, p) == cudaSuccess;
+    if (args.after_quantizer) config.numAttrs = 2;
+    return cudaLaunchKernelEx(&config, &small_kernel<T, kBackward, kOutBf16>, map_a, map_w, p) == cudaSuccess;
 }
 
 template <bool kBackward, bool kOutBf16>
-bool launch_small(const Args& args, int tokens, int splits) {
-    switch (tokens) {
-        case 16: return launch_small_instance<16, kBackward, kOutBf16>(args, splits);
-        case 32: return launch_small_instance<32, kBackward, kOutBf16>(args, splits);
-        case 64: return launch_small_instance<64, kBackward, kOutBf16>(args, splits);
-        default: return launch_small_instance<128, kBackward, kOutBf16>(args, splits);
-    }
-}
-
-template <bool kBackward, bool kOutBf16>
-bool launch_pair(const Args& args, int tile_n) {
+bool launch_pair(const Args& args) {
     using L = PairSmem;
     auto* const kernel = &pair_kernel<kBackward, kOutBf16>;
     static PerDeviceState resident_pairs;
@@ -824,21 +857,20 @@ bool launch_pair(const Args& args, int tile_n) {
     });
     if (pairs <= 0) return false;
     CUtensorMap map_a, map_w, map_c;
-    if (!make_maps(args, 128, kBackward ? 128 : tile_n / 2, map_a, map_w)) return false;
+    if (!make_maps(args, 128, kBackward ? 128 : kPairN / 2, map_a, map_w)) return false;
     const uint64_t c_dims[2] = {static_cast<uint64_t>(args.width()), static_cast<uint64_t>(args.M)};
     const uint64_t c_strides[1] = {static_cast<uint64_t>(args.width()) * 2};
     const uint32_t c_box[2] = {32, 32};
     if (!encode_map(&map_c, kOutBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, args.c, c_dims, c_strides, c_box, CU_TENSOR_MAP_SWIZZLE_64B)) return false;
     Params p = make_params(args);
-    const int64_t tiles_m = (args.M + 255) / 256, tiles_n = (args.width() + tile_n - 1) / tile_n;
+    const int64_t tiles_m = (args.M + 255) / 256, tiles_n = (args.width() + kPairN - 1) / kPairN;
     if (tiles_m * tiles_n > 0x7fffffff) return false;
     p.tiles_m = static_cast<int>(tiles_m);
     p.tiles_n = static_cast<int>(tiles_n);
-    p.tile_n = tile_n;
     int64_t band = (32ll << 20) / (256 * args.depth());   // about 32 MB of activations stay in L2 while a band sweeps the weight
     if (band < 4) band = 4;
     p.band = static_cast<int>(band < tiles_m ? band : tiles_m);
-    p.idesc = make_idesc(kAccF32, format(args.a_e5m2), format(args.w_e5m2), 256, static_cast<uint32_t>(tile_n / 2)) | (kBackward ? kIdescBMajorMN : 0u);
+    p.idesc = make_idesc(kAccF32, format(args.a_e5m2), format(args.w_e5m2), 256, static_cast<uint32_t>(kPairN / 2)) | (kBackward ? kIdescBMajorMN : 0u);
     cudaLaunchConfig_t config = {};
     const int64_t tiles = tiles_m * tiles_n;
     config.gridDim = dim3(static_cast<unsigned>(2 * (tiles < pairs ? tiles : pairs)));
@@ -853,28 +885,47 @@ bool launch_pair(const Args& args, int tile_n) {
     return cudaLaunchKernelEx(&config, kernel, map_a, map_w, map_c, p) == cudaSuccess;
 }
 
-// Which kernel a product gets.
-struct Plan {
-    int tokens;   // small kernel: tokens per tile; 0: pair kernel
-    int splits;   // small kernel: K splits, at most 8
-    int tile_n;   // pair kernel: outputs per tile
-};
-
-Plan plan(int64_t M, int64_t width, int64_t depth, int sms) {
-    const int64_t num_kb = (depth + kBlock - 1) / kBlock;
-    const int64_t pair_tiles = (M + 255) / 256 * ((width + 255) / 256);
-    if (M > 128 && pair_tiles * 4 >= sms) return {0, 1, 256};
-    const int tokens = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-    const int64_t tiles = (M + tokens - 1) / tokens * ((width + 127) / 128);
-    int splits = 1;
-    while (splits < 8 && tiles * splits * 2 <= 2 * sms && num_kb >= 4 * splits) splits *= 2;
-    return {tokens, splits, 0};
+// Microseconds that a product takes on the small kernel with T tokens per tile and `splits` K splits, or a negative number
+// where the clusters would not be resident at once. Per launch 3.5; per k block of a CTA 0.29 with 16 or 32 tokens and 0.45 with
+// 128 (every SM busy; the activation tile then is as large as the weight's); the exchange of the partial sums 1.0 and 1.8.
+template <int T, bool kBackward, bool kOutBf16>
+double small_cost(const Args& args, int splits) {
+    const int64_t num_kb = (args.depth() + kBlock - 1) / kBlock;
+    const int64_t tiles = (args.M + T - 1) / T * ((args.width() + 127) / 128);
+    const int clusters = splits > num_kb ? 0 : small_clusters<T, kBackward, kOutBf16>(splits);
+    if (clusters <= 0 || (splits > 1 && tiles > clusters)) return -1.0;
+    const double rounds = static_cast<double>((tiles + clusters - 1) / clusters);
+    return 3.5 + rounds * static_cast<double>((num_kb + splits - 1) / splits) * (T == 128 ? 0.45 : 0.29) + (splits == 1 ? 0.0 : T == 128 ? 1.8 : 1.0);
 }
 
+template <int T, bool kBackward, bool kOutBf16>
+bool launch_best_small(const Args& args, double pair_cost) {
+    int best = 1;
+    double best_cost = small_cost<T, kBackward, kOutBf16>(args, 1);
+    for (int splits = 2; splits <= kMaxSplits; ++splits) {
+        const double cost = small_cost<T, kBackward, kOutBf16>(args, splits);
+        if (cost >= 0.0 && cost < best_cost) {
+            best = splits;
+            best_cost = cost;
+        }
+    }
+    if (best_cost > pair_cost) return launch_pair<kBackward, kOutBf16>(args);
+    return launch_small<T, kBackward, kOutBf16>(args, best);
+}
+
+// Up to 16 and 32 tokens their own tiles, above that 128 tokens per tile or the pair kernel, whichever the model says: a round of the
+// pair kernel's tiles costs 0.57 us per k block and 1 us for its end (512 x 4096 x 4096: 17.7 us small, 21.1 pair; 1024 x 4096 x 4096:
+// 33.7 against 22.2; 777 x 3856 x 2576: 26.6 against 16.3; 300 x 12288 x 4096: 33.8 against 37.5).
 template <bool kBackward, bool kOutBf16>
 bool launch(const Args& args) {
-    const Plan pick = plan(args.M, args.width(), args.depth(), device_info().sm_count);
-    return pick.tokens == 0 ? launch_pair<kBackward, kOutBf16>(args, pick.tile_n) : launch_small<kBackward, kOutBf16>(args, pick.tokens, pick.splits);
+    constexpr double kNever = 1e30;
+    if (args.M <= 16) return launch_best_small<16, kBackward, kOutBf16>(args, kNever);
+    if (args.M <= 32) return launch_best_small<32, kBackward, kOutBf16>(args, kNever);
+    const int pairs = device_info().sm_count / 2;
+    const int64_t tiles = (args.M + 255) / 256 * ((args.width() + kPairN - 1) / kPairN);
+    const int64_t num_kb = (args.depth() + kBlock - 1) / kBlock;
+    const double pair_cost = 4.0 + static_cast<double>((tiles + pairs - 1) / pairs) * (0.57 * static_cast<double>(num_kb) + 1.0);
+    return launch_best_small<128, kBackward, kOutBf16>(args, pair_cost);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
