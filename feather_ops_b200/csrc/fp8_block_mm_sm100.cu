@@ -23,6 +23,10 @@
 #include "sm100_ptx.cuh"
 
 namespace feather {
+
+// The activation quantizer as an ordinary launch that signals its dependents (fp8_block_quantize_sm100.cu).
+bool launch_fp8_block_quantize_ahead(const void* x, void* q, float* scale, int64_t M, int64_t K, int input_fp16, int use_e5m2, cudaStream_t stream);
+
 namespace f8mm {
 
 constexpr int kBlock = 128;          // depth of a k block = channels per scale
@@ -42,6 +46,7 @@ struct Params {
     int tiles_m, tiles_n;
     int splits;              // small kernel: CTAs of a cluster along the contraction
     int band;                // pair kernel: row tiles per band of the walk
+    bool weight_ready;       // small kernel: the weight may be read before the kernel ahead has finished
     uint32_t idesc;
 };
 
@@ -232,15 +237,20 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
     if (warp == L::kWarps) {
         // ---------------------------------------------------------------------- loads
         if (elect_one()) {
+            const auto load_weight = [&](int i, int slot) {
+                const int depth0 = (kb_begin + i) * kBlock;
+                mbar_arrive_expect_tx(&full[slot], L::kStageBytes);
+                tma_load_2d(smem + slot * L::kStageBytes, &map_w, &full[slot], kBackward ? n0 : depth0, kBackward ? depth0 : n0);
+            };
+            // behind the quantizer the weight fills the ring while that runs
+            const int early = p.weight_ready ? (blocks < L::kStages ? blocks : L::kStages) : 0;
+            for (int i = 0; i < early; ++i) load_weight(i, i);
             grid_dependency_wait();
             Ring slot;
             for (int i = 0; i < blocks; ++i) {
-                const int depth0 = (kb_begin + i) * kBlock;
                 if (!guard.wait(&empty[slot.idx], slot.phase ^ 1u, kSiteLoadEmpty)) break;
-                uint8_t* const w_tile = smem + slot.idx * L::kStageBytes;
-                mbar_arrive_expect_tx(&full[slot.idx], L::kStageBytes);
-                tma_load_2d(w_tile, &map_w, &full[slot.idx], kBackward ? n0 : depth0, kBackward ? depth0 : n0);
-                tma_load_2d(w_tile + kTileBytes, &map_a, &full[slot.idx], depth0, m0);
+                if (i >= early) load_weight(i, static_cast<int>(slot.idx));
+                tma_load_2d(smem + slot.idx * L::kStageBytes + kTileBytes, &map_a, &full[slot.idx], (kb_begin + i) * kBlock, m0);
                 slot.advance(L::kStages);
             }
         }
@@ -727,7 +737,9 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// Launch
+// Launch. Both kernels are programmatic dependents: they may start while the kernel ahead in the stream ends, and wait for it
+// (griddepcontrol.wait) before they read what it may have written. That is everything, except in the call that quantizes and
+// multiplies: its quantizer is an ordinary launch, so by the time it runs nothing older can still write the weight.
 // ---------------------------------------------------------------------------------------------------------
 struct Args {
     const uint8_t* a;
@@ -738,7 +750,7 @@ struct Args {
     uint16_t* c;
     int64_t M, N, K;   // N and K: the weight's axes
     bool transposed_b, a_e5m2, w_e5m2, out_bf16;
-    bool after_quantizer;   // the kernel before this one in the stream signals its dependents
+    bool weight_ready;   // the kernel ahead in the stream is this library's quantizer, launched in the same call after all else had finished
     cudaStream_t stream;
 
     int64_t width() const { return transposed_b ? K : N; }
@@ -819,6 +831,7 @@ bool launch_small(const Args& args, int splits) {
     p.tiles_m = static_cast<int>(tiles_m);
     p.tiles_n = static_cast<int>(tiles_n);
     p.splits = splits;
+    p.weight_ready = args.weight_ready;
     p.idesc = SmallShape<T>::kTokenLanes ? make_idesc(kAccF32, format(args.a_e5m2), format(args.w_e5m2), 128, 128) | (kBackward ? kIdescBMajorMN : 0u)
                                          : make_idesc(kAccF32, format(args.w_e5m2), format(args.a_e5m2), 128, T) | (kBackward ? kIdescAMajorMN : 0u);
     cudaLaunchAttribute attr[2];
@@ -826,7 +839,7 @@ bool launch_small(const Args& args, int splits) {
     config.stream = args.stream;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
-    if (args.after_quantizer) config.numAttrs = 2;
+    config.numAttrs = 2;
     return cudaLaunchKernelEx(&config, &small_kernel<T, kBackward, kOutBf16>, map_a, map_w, p) == cudaSuccess;
 }
 
@@ -881,7 +894,7 @@ bool launch_pair(const Args& args) {
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     config.attrs = attr;
-    config.numAttrs = args.after_quantizer ? 1 : 0;
+    config.numAttrs = 1;
     return cudaLaunchKernelEx(&config, kernel, map_a, map_w, map_c, p) == cudaSuccess;
 }
 
@@ -930,22 +943,39 @@ bool launch(const Args& args) {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+bool valid(const Args& args) {
+    constexpr int64_t kMost = 1 << 30;
+    if (args.M < 0 || args.N <= 0 || args.K <= 0 || args.M > kMost || args.N > kMost || args.K > kMost || args.N % 16 != 0 || args.K % 16 != 0) return false;
+    if (args.transposed_b && args.bias != nullptr) return false;
+    if (args.M == 0) return true;
+    if (args.a == nullptr || args.a_scale == nullptr || args.w == nullptr || args.w_scale == nullptr || args.c == nullptr) return false;
+    return aligned16(args.a) && aligned16(args.w) && aligned16(args.c);
+}
+
+bool launch(const Args& args) {
+    if (args.M == 0) return true;
+    if (args.transposed_b) return args.out_bf16 ? launch<true, true>(args) : launch<true, false>(args);
+    return args.out_bf16 ? launch<false, true>(args) : launch<false, false>(args);
+}
+
 }  // namespace f8mm
 }  // namespace feather
 
 extern "C" bool launch_fp8_block_mm(const uint8_t* a, const float* a_scale, const uint8_t* w, const float* w_scale, const uint16_t* bias, uint16_t* c,
                                     int64_t M, int64_t N, int64_t K, bool transposed_b, int a_e5m2, int w_e5m2, int output_dtype, cudaStream_t stream) {
     using namespace feather::f8mm;
-    constexpr int64_t kMost = 1 << 30;
-    if (M < 0 || N <= 0 || K <= 0 || M > kMost || N > kMost || K > kMost || N % 16 != 0 || K % 16 != 0) return false;
-    if (transposed_b && bias != nullptr) return false;
     if (output_dtype != 0 && output_dtype != 1) return false;
-    if (M == 0) return true;
-    if (a == nullptr || a_scale == nullptr || w == nullptr || w_scale == nullptr || c == nullptr) return false;
-    if (!aligned16(a) || !aligned16(w) || !aligned16(c)) return false;
     const Args args{a, a_scale, w, w_scale, bias, c, M, N, K, transposed_b, a_e5m2 != 0, w_e5m2 != 0, output_dtype == 1, false, stream};
-    if (transposed_b) return args.out_bf16 ? launch<true, true>(args) : launch<true, false>(args);
-    return args.out_bf16 ? launch<false, true>(args) : launch<false, false>(args);
+    return valid(args) && launch(args);
+}
+
+extern "C" bool launch_fp8_block_linear(const void* x, uint8_t* q, float* q_scale, const uint8_t* w, const float* w_scale, const uint16_t* bias, uint16_t* c,
+                                        int64_t M, int64_t N, int64_t K, bool transposed_b, int input_fp16, int q_e5m2, int w_e5m2, int output_dtype,
+                                        cudaStream_t stream) {
+    using namespace feather::f8mm;
+    if (output_dtype != 0 && output_dtype != 1) return false;
+    const Args args{q, q_scale, w, w_scale, bias, c, M, N, K, transposed_b, q_e5m2 != 0, w_e5m2 != 0, output_dtype == 1, true, stream};
+    return valid(args) && feather::launch_fp8_block_quantize_ahead(x, q, q_scale, M, args.depth(), input_fp16, q_e5m2, stream) && launch(args);
 }
 
 // Reads and clears the product's wait-status record (see feather_scaled_mm_status).

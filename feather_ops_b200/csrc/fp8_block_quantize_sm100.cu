@@ -8,6 +8,9 @@
 // or a NaN gets a scale that is not finite and never reads back as ordinary numbers.
 // The scales are laid out [ceil(K / 128), M]: the product's epilogue wants the scales of consecutive rows at one block.
 //
+// Every kernel may start while the one ahead in its stream ends (programmatic dependent launch), waits for it before it
+// reads or writes memory, and lets the next one start likewise.
+//
 // All five kernels are bound by HBM: a thread moves 8 consecutive channels (one 16-byte load, one 8-byte store of codes),
 // 16 lanes hold one block, and its maximum is four shuffles.
 #include <cuda_bf16.h>
@@ -18,6 +21,7 @@
 #include <cstdint>
 
 #include "feather_host.h"
+#include "sm100_ptx.cuh"
 
 namespace feather {
 namespace {
@@ -88,6 +92,12 @@ __device__ __forceinline__ uint2 encode_block(const float (&v)[kVec], float& sca
     return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
 }
 
+// The next kernel's blocks are let in at once (they take what room is left and wait as this one does), then this one waits.
+__device__ __forceinline__ void start_after_kernel_ahead() {
+    grid_launch_dependents();
+    grid_dependency_wait();
+}
+
 __device__ __forceinline__ uint4 load16(const uint16_t* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
 
 __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
@@ -101,6 +111,7 @@ constexpr int kTileWarps = 8;
 template <bool kFp16, bool kE5M2, bool kGate, int kRows>
 __global__ void __launch_bounds__(32 * kTileWarps) tile_quantize_kernel(const uint16_t* __restrict__ x, uint8_t* __restrict__ q,
                                                                         float* __restrict__ scale, int64_t M, int64_t K, int column_warps) {
+    start_after_kernel_ahead();
     const int lane = threadIdx.x & 31;
     const int64_t task = static_cast<int64_t>(blockIdx.x) * kTileWarps + (threadIdx.x >> 5);
     const int64_t row0 = task / column_warps * kRows;
@@ -139,6 +150,7 @@ __global__ void __launch_bounds__(32 * kTileWarps) tile_quantize_kernel(const ui
 template <bool kFp16>
 __global__ void __launch_bounds__(256) silu_mul_dgrad_kernel(const uint16_t* __restrict__ grad, const uint16_t* __restrict__ gate_up,
                                                              uint16_t* __restrict__ out, int64_t chunks, int64_t row_chunks) {
+    start_after_kernel_ahead();
     const int64_t chunk = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     if (chunk >= chunks) return;
     const int64_t row = chunk / row_chunks;
@@ -211,6 +223,7 @@ struct NormParams {
 template <bool kFp16, bool kWeightF32, bool kE5M2, int kChunks>
 __global__ void __launch_bounds__(kMaxNormThreads) rms_norm_fp8_kernel(const NormParams p) {
     __shared__ float slots[32];
+    start_after_kernel_ahead();
     const int64_t row = blockIdx.x;
     const int64_t base = row * p.K;
     const int step = blockDim.x * kVec;
@@ -287,6 +300,7 @@ struct NormGradParams {
 template <bool kFp16, bool kWeightF32, int kChunks>
 __global__ void __launch_bounds__(kMaxNormThreads) rms_norm_dgrad_kernel(const NormGradParams p) {
     __shared__ float slots[32];
+    start_after_kernel_ahead();
     const int step = blockDim.x * kVec;
     float dw[kChunks][kVec];
 #pragma unroll
@@ -357,6 +371,7 @@ __global__ void __launch_bounds__(kMaxNormThreads) rms_norm_dgrad_kernel(const N
 constexpr int kSumWarps = 8;
 __global__ void __launch_bounds__(32 * kSumWarps) column_sum_kernel(const float* __restrict__ partials, float* __restrict__ out, int rows, int64_t K) {
     __shared__ float part[kSumWarps][33];
+    start_after_kernel_ahead();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t column = static_cast<int64_t>(blockIdx.x) * 32 + lane;
     float sum = 0.0f;
@@ -371,7 +386,20 @@ __global__ void __launch_bounds__(32 * kSumWarps) column_sum_kernel(const float*
     }
 }
 
-bool launched() { return cudaGetLastError() == cudaSuccess; }
+// `overlap`: may start while the kernel ahead in the stream still runs
+template <class... Params, class... Args>
+bool launch_kernel(void (*kernel)(Params...), int64_t grid, int threads, cudaStream_t stream, bool overlap, Args... args) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(static_cast<unsigned>(grid));
+    config.blockDim = dim3(static_cast<unsigned>(threads));
+    config.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attr;
+    config.numAttrs = overlap ? 1 : 0;
+    return cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...) == cudaSuccess;
+}
 
 bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
@@ -391,25 +419,24 @@ RowShape row_shape(int64_t M, int64_t K, int wanted) {
 }
 
 template <bool kFp16, bool kE5M2, bool kGate>
-bool launch_tile(const void* x, void* q, float* scale, int64_t M, int64_t K, cudaStream_t stream) {
+bool launch_tile(const void* x, void* q, float* scale, int64_t M, int64_t K, cudaStream_t stream, bool overlap) {
     const int64_t column_warps = (K + kWarpChannels - 1) / kWarpChannels;
     const int rows = M * column_warps > 16LL * device_info().sm_count * kTileWarps ? 4 : 1;
     const int64_t tasks = (M + rows - 1) / rows * column_warps;
     const int64_t grid = (tasks + kTileWarps - 1) / kTileWarps;
     if (column_warps > 0x7fffffff || grid > 0x7fffffff) return false;
     const auto kernel = rows == 4 ? tile_quantize_kernel<kFp16, kE5M2, kGate, 4> : tile_quantize_kernel<kFp16, kE5M2, kGate, 1>;
-    kernel<<<static_cast<unsigned>(grid), 32 * kTileWarps, 0, stream>>>(static_cast<const uint16_t*>(x), static_cast<uint8_t*>(q), scale, M, K,
-                                                                        static_cast<int>(column_warps));
-    return launched();
+    return launch_kernel(kernel, grid, 32 * kTileWarps, stream, overlap, static_cast<const uint16_t*>(x), static_cast<uint8_t*>(q), scale, M, K,
+                         static_cast<int>(column_warps));
 }
 
 template <bool kGate>
-bool dispatch_tile(const void* x, void* q, float* scale, int64_t M, int64_t K, bool fp16, bool e5m2, cudaStream_t stream) {
+bool dispatch_tile(const void* x, void* q, float* scale, int64_t M, int64_t K, bool fp16, bool e5m2, cudaStream_t stream, bool overlap = true) {
     if (M < 0 || K <= 0 || K % 16 != 0) return false;
     if (M == 0) return true;
     if (x == nullptr || q == nullptr || scale == nullptr || !aligned(x, 16) || !aligned(q, 16) || !aligned(scale, 4)) return false;
-    if (fp16) return e5m2 ? launch_tile<true, true, kGate>(x, q, scale, M, K, stream) : launch_tile<true, false, kGate>(x, q, scale, M, K, stream);
-    return e5m2 ? launch_tile<false, true, kGate>(x, q, scale, M, K, stream) : launch_tile<false, false, kGate>(x, q, scale, M, K, stream);
+    if (fp16) return e5m2 ? launch_tile<true, true, kGate>(x, q, scale, M, K, stream, overlap) : launch_tile<true, false, kGate>(x, q, scale, M, K, stream, overlap);
+    return e5m2 ? launch_tile<false, true, kGate>(x, q, scale, M, K, stream, overlap) : launch_tile<false, false, kGate>(x, q, scale, M, K, stream, overlap);
 }
 
 template <bool kFp16, bool kWeightF32, bool kE5M2>
@@ -418,8 +445,7 @@ bool launch_norm(const NormParams& p, cudaStream_t stream) {
     const auto kernel = shape.chunks == 1   ? rms_norm_fp8_kernel<kFp16, kWeightF32, kE5M2, 1>
                         : shape.chunks == 2 ? rms_norm_fp8_kernel<kFp16, kWeightF32, kE5M2, 2>
                                             : rms_norm_fp8_kernel<kFp16, kWeightF32, kE5M2, 4>;
-    kernel<<<static_cast<unsigned>(p.M), shape.threads, 0, stream>>>(p);
-    return launched();
+    return launch_kernel(kernel, p.M, shape.threads, stream, true, p);
 }
 
 template <bool kFp16, bool kWeightF32>
@@ -428,8 +454,7 @@ bool launch_norm_grad(const NormGradParams& p, int grid, cudaStream_t stream) {
     const auto kernel = shape.chunks == 1   ? rms_norm_dgrad_kernel<kFp16, kWeightF32, 1>
                         : shape.chunks == 2 ? rms_norm_dgrad_kernel<kFp16, kWeightF32, 2>
                                             : rms_norm_dgrad_kernel<kFp16, kWeightF32, 4>;
-    kernel<<<grid, shape.threads, 0, stream>>>(p);
-    return launched();
+    return launch_kernel(kernel, grid, shape.threads, stream, true, p);
 }
 
 // CTAs of the norm's backward pass: at most two per SM of a B200 (their registers hold two), at least four rows each. A
@@ -441,6 +466,11 @@ int norm_grad_grid(int64_t M) {
 }
 
 }  // namespace
+
+bool launch_fp8_block_quantize_ahead(const void* x, void* q, float* scale, int64_t M, int64_t K, int input_fp16, int use_e5m2, cudaStream_t stream) {
+    return dispatch_tile<false>(x, q, scale, M, K, input_fp16 != 0, use_e5m2 != 0, stream, false);
+}
+
 }  // namespace feather
 
 using namespace feather;
@@ -466,9 +496,8 @@ extern "C" bool launch_silu_mul_dgrad(const void* grad, const void* gate_up, voi
     const int64_t grid = (chunks + 255) / 256;
     if (grid > 0x7fffffff) return false;
     const auto kernel = input_fp16 != 0 ? silu_mul_dgrad_kernel<true> : silu_mul_dgrad_kernel<false>;
-    kernel<<<static_cast<unsigned>(grid), 256, 0, stream>>>(static_cast<const uint16_t*>(grad), static_cast<const uint16_t*>(gate_up),
-                                                                                       static_cast<uint16_t*>(grad_gate_up), chunks, row_chunks);
-    return launched();
+    return launch_kernel(kernel, grid, 256, stream, true, static_cast<const uint16_t*>(grad), static_cast<const uint16_t*>(gate_up),
+                         static_cast<uint16_t*>(grad_gate_up), chunks, row_chunks);
 }
 
 extern "C" bool launch_rms_norm_fp8(const void* x, const void* residual, const void* weight, void* residual_out, void* q, float* scale, float* rstd,
@@ -512,6 +541,5 @@ extern "C" bool launch_rms_norm_dgrad(const void* grad, const void* x, const voi
         ok = weight_f32 != 0 ? launch_norm_grad<false, true>(p, grid, stream) : launch_norm_grad<false, false>(p, grid, stream);
     }
     if (!ok) return false;
-    column_sum_kernel<<<static_cast<unsigned>((K + 31) / 32), 32 * kSumWarps, 0, stream>>>(partials, grad_weight, grid, K);
-    return launched();
+    return launch_kernel(column_sum_kernel, (K + 31) / 32, 32 * kSumWarps, stream, true, static_cast<const float*>(partials), grad_weight, grid, K);
 }

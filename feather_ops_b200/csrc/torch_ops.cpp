@@ -3,7 +3,8 @@
 // csrc/hip_conv2d_3x3.cu:672-692), `scaled_mm_splitk` (the skinny-M launcher over caller scratch) and the block-scaled
 // fp8 operators (neither has a counterpart in the reference). It validates tensors with the reference's messages, takes the current
 // CUDA stream of the input's device and forwards raw pointers to libfeather_ops_b200.so. Built against
-// torch's stable ABI, so it does not depend on libtorch_python. Nothing here computes or allocates.
+// torch's stable ABI, so it does not depend on libtorch_python. Nothing here computes, and only the block-scaled operators
+// allocate.
 #include <Python.h>
 
 #include <torch/csrc/inductor/aoti_torch/c/shim.h>
@@ -14,7 +15,10 @@
 #include <torch/headeronly/util/Exception.h>
 
 #include <cstdint>
+#include <initializer_list>
 #include <optional>
+#include <tuple>
+#include <utility>
 
 #include "feather_ops_b200.h"
 
@@ -319,20 +323,27 @@ void convrot_quantize(const Tensor& x, const std::optional<Tensor>& col_scale, T
     STD_TORCH_CHECK(ok, "convrot_quantize launch failed");
 }
 
+// ---------------------------------------------------------------------------------------------------------
+// The block-scaled fp8 operators (no counterpart in the reference). They allocate what they return: a call of a few tokens
+// is a few microseconds on the device, and every tensor that Python allocates costs about two. `scale` of an activation is
+// [ceil(K / 128), M].
+// ---------------------------------------------------------------------------------------------------------
 bool is_fp8(ScalarType t) { return t == ScalarType::Float8_e4m3fn || t == ScalarType::Float8_e5m2; }
 
-// The block-scaled fp8 operators (no counterpart in the reference). `scale` of an activation is [ceil(K / 128), M].
-void check_block_codes(const Tensor& q, const Tensor& scale, int64_t M, int64_t K, int32_t device) {
-    STD_TORCH_CHECK(q.is_cuda() && scale.is_cuda() && q.get_device_index() == device && scale.get_device_index() == device,
-                    "the codes and their scales must be on the input's CUDA device");
-    STD_TORCH_CHECK(is_fp8(q.scalar_type()), "the codes must be float8_e4m3fn or float8_e5m2");
-    STD_TORCH_CHECK(scale.scalar_type() == ScalarType::Float, "the block scales must be float32");
-    STD_TORCH_CHECK(K > 0 && K % 16 == 0, "the row length must be a positive multiple of 16");
-    STD_TORCH_CHECK(q.dim() == 2 && q.size(0) == M && q.size(1) == K, "the codes must be [", M, ", ", K, "]");
-    STD_TORCH_CHECK(scale.dim() == 2 && scale.size(0) == (K + 127) / 128 && scale.size(1) == M, "the block scales must be [", (K + 127) / 128, ", ", M, "]");
-    STD_TORCH_CHECK(q.is_contiguous() && scale.is_contiguous(), "the codes and their scales must be contiguous");
-    STD_TORCH_CHECK(aligned16(q.const_data_ptr()), "the codes' data pointer must be 16-byte aligned");
+int64_t blocks_of(int64_t size) { return (size + 127) / 128; }
+
+// An uninitialised tensor on a CUDA device, of the caching allocator and its current stream.
+Tensor make_empty(std::initializer_list<int64_t> sizes, int32_t dtype, int32_t device) {
+    int64_t strides[2] = {1, 1};
+    if (sizes.size() == 2) strides[0] = sizes.begin()[1] > 0 ? sizes.begin()[1] : 1;
+    AtenTensorHandle handle = nullptr;
+    TORCH_ERROR_CODE_CHECK(aoti_torch_empty_strided(static_cast<int64_t>(sizes.size()), sizes.begin(), strides, dtype, aoti_torch_device_type_cuda(), device, &handle));
+    return Tensor(handle);
 }
+
+int32_t code_dtype(bool e5m2) { return e5m2 ? aoti_torch_dtype_float8_e5m2() : aoti_torch_dtype_float8_e4m3fn(); }
+int32_t half_dtype(bool fp16) { return fp16 ? aoti_torch_dtype_float16() : aoti_torch_dtype_bfloat16(); }
+bool is_half(const Tensor& t) { return t.scalar_type() == ScalarType::Half; }
 
 // A 16-bit matrix [M, K] that a row-wise kernel reads or writes, of dtype `type` on `device`.
 void check_rows(const Tensor& t, const char* name, int64_t M, int64_t K, ScalarType type, int32_t device) {
@@ -343,52 +354,93 @@ void check_rows(const Tensor& t, const char* name, int64_t M, int64_t K, ScalarT
     STD_TORCH_CHECK(aligned16(t.const_data_ptr()), name, " data pointer must be 16-byte aligned");
 }
 
-void fp8_block_quantize(const Tensor& x, Tensor& q, Tensor& scale) {
-    STD_TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
-    STD_TORCH_CHECK(is_half_or_bf16(x.scalar_type()), "x must be float16 or bfloat16");
-    STD_TORCH_CHECK(x.dim() == 2, "x must be 2D");
-    const auto device = x.get_device_index();
-    const int64_t M = x.size(0), K = x.size(1);
-    check_rows(x, "x", M, K, x.scalar_type(), device);
-    check_block_codes(q, scale, M, K, device);
-    torch::stable::accelerator::DeviceGuard guard(device);
-    const bool ok = launch_fp8_block_quantize(x.const_data_ptr(), q.mutable_data_ptr(), static_cast<float*>(scale.mutable_data_ptr()), M, K,
-                                              x.scalar_type() == ScalarType::Half ? 1 : 0, q.scalar_type() == ScalarType::Float8_e5m2 ? 1 : 0,
-                                              current_stream(device));
-    STD_TORCH_CHECK(ok, "fp8_block_quantize launch failed");
+// The first 16-bit input of a row-wise operator, [M, width]; `unit`: what the width must be a multiple of.
+void check_input(const Tensor& x, const char* name, int64_t unit) {
+    STD_TORCH_CHECK(x.is_cuda(), name, " must be a CUDA tensor");
+    STD_TORCH_CHECK(is_half_or_bf16(x.scalar_type()), name, " must be float16 or bfloat16");
+    STD_TORCH_CHECK(x.dim() == 2, name, " must be 2D");
+    STD_TORCH_CHECK(x.size(1) > 0 && x.size(1) % unit == 0, name, "'s row length must be a positive multiple of ", unit);
+    STD_TORCH_CHECK(x.is_contiguous(), name, " must be contiguous");
+    STD_TORCH_CHECK(aligned16(x.const_data_ptr()), name, " data pointer must be 16-byte aligned");
 }
 
-void fp8_block_mm(const Tensor& a, const Tensor& a_scale, const Tensor& weight, const Tensor& weight_scale, const std::optional<Tensor>& bias, Tensor& c,
-                  bool transposed_b) {
-    STD_TORCH_CHECK(a.is_cuda() && weight.is_cuda() && weight_scale.is_cuda() && c.is_cuda(), "tensors must be CUDA tensors");
-    const auto device = a.get_device_index();
-    STD_TORCH_CHECK(weight.get_device_index() == device && weight_scale.get_device_index() == device && c.get_device_index() == device,
-                    "tensors must be on the same device");
+std::tuple<Tensor, Tensor> fp8_block_quantize(const Tensor& x, bool e5m2) {
+    check_input(x, "x", 16);
+    const auto device = x.get_device_index();
+    const int64_t M = x.size(0), K = x.size(1);
+    torch::stable::accelerator::DeviceGuard guard(device);
+    Tensor q = make_empty({M, K}, code_dtype(e5m2), device);
+    Tensor scale = make_empty({blocks_of(K), M}, aoti_torch_dtype_float32(), device);
+    const bool ok = launch_fp8_block_quantize(x.const_data_ptr(), q.mutable_data_ptr(), static_cast<float*>(scale.mutable_data_ptr()), M, K, is_half(x) ? 1 : 0,
+                                              e5m2 ? 1 : 0, current_stream(device));
+    STD_TORCH_CHECK(ok, "fp8_block_quantize launch failed");
+    return std::make_tuple(std::move(q), std::move(scale));
+}
+
+// What a product needs of its weight and bias.
+void check_block_weight(const Tensor& weight, const Tensor& weight_scale, const std::optional<Tensor>& bias, bool out_fp16, bool transposed_b, int32_t device) {
+    STD_TORCH_CHECK(weight.is_cuda() && weight_scale.is_cuda(), "tensors must be CUDA tensors");
+    STD_TORCH_CHECK(weight.get_device_index() == device && weight_scale.get_device_index() == device, "tensors must be on the same device");
     STD_TORCH_CHECK(is_fp8(weight.scalar_type()), "weight must be float8_e4m3fn or float8_e5m2");
-    STD_TORCH_CHECK(is_half_or_bf16(c.scalar_type()), "c must be float16 or bfloat16");
-    STD_TORCH_CHECK(a.dim() == 2 && weight.dim() == 2 && c.dim() == 2, "a, weight and c must be 2D");
-    const int64_t M = a.size(0), N = weight.size(0), K = weight.size(1);
+    STD_TORCH_CHECK(weight.dim() == 2, "weight must be 2D");
+    const int64_t N = weight.size(0), K = weight.size(1);
     STD_TORCH_CHECK(N > 0 && K > 0 && N % 16 == 0 && K % 16 == 0, "the weight axes must be positive multiples of 16");
-    STD_TORCH_CHECK(a.size(1) == (transposed_b ? N : K), "a's row length must equal the weight axis that is contracted");
-    check_block_codes(a, a_scale, M, a.size(1), device);
     STD_TORCH_CHECK(weight_scale.scalar_type() == ScalarType::Float, "weight_scale must be float32");
-    STD_TORCH_CHECK(weight_scale.dim() == 2 && weight_scale.size(0) == (N + 127) / 128 && weight_scale.size(1) == (K + 127) / 128,
-                    "weight_scale must be [", (N + 127) / 128, ", ", (K + 127) / 128, "]");
-    STD_TORCH_CHECK(c.size(0) == M && c.size(1) == (transposed_b ? K : N), "c has the wrong shape");
-    STD_TORCH_CHECK(weight.is_contiguous() && weight_scale.is_contiguous() && c.is_contiguous(), "weight, weight_scale and c must be contiguous");
+    STD_TORCH_CHECK(weight_scale.dim() == 2 && weight_scale.size(0) == blocks_of(N) && weight_scale.size(1) == blocks_of(K), "weight_scale must be [",
+                    blocks_of(N), ", ", blocks_of(K), "]");
+    STD_TORCH_CHECK(weight.is_contiguous() && weight_scale.is_contiguous(), "weight and weight_scale must be contiguous");
+    STD_TORCH_CHECK(aligned16(weight.const_data_ptr()), "weight data pointer must be 16-byte aligned");
     STD_TORCH_CHECK(!transposed_b || !bias.has_value(), "transposed_b takes no bias");
     if (bias.has_value()) {
-        STD_TORCH_CHECK(bias->is_cuda() && bias->scalar_type() == c.scalar_type() && bias->get_device_index() == device, "bias must have c's dtype and device");
+        STD_TORCH_CHECK(bias->is_cuda() && bias->get_device_index() == device, "bias must be on the same device");
+        STD_TORCH_CHECK(bias->scalar_type() == (out_fp16 ? ScalarType::Half : ScalarType::BFloat16), "bias must have the output's dtype");
         STD_TORCH_CHECK(bias->numel() == N && bias->is_contiguous(), "bias must have N contiguous elements");
     }
-    STD_TORCH_CHECK(aligned16(weight.const_data_ptr()) && aligned16(c.mutable_data_ptr()), "data pointers must be 16-byte aligned");
+}
+
+const uint16_t* bias_ptr(const std::optional<Tensor>& bias) { return bias.has_value() ? static_cast<const uint16_t*>(bias->const_data_ptr()) : nullptr; }
+
+Tensor fp8_block_mm(const Tensor& a, const Tensor& a_scale, const Tensor& weight, const Tensor& weight_scale, const std::optional<Tensor>& bias, bool out_fp16,
+                    bool transposed_b) {
+    STD_TORCH_CHECK(a.is_cuda(), "a must be a CUDA tensor");
+    STD_TORCH_CHECK(is_fp8(a.scalar_type()), "a must be float8_e4m3fn or float8_e5m2");
+    STD_TORCH_CHECK(a.dim() == 2, "a must be 2D");
+    const auto device = a.get_device_index();
+    check_block_weight(weight, weight_scale, bias, out_fp16, transposed_b, device);
+    const int64_t M = a.size(0), N = weight.size(0), K = weight.size(1), depth = transposed_b ? N : K;
+    STD_TORCH_CHECK(a.size(1) == depth, "a's row length must equal the weight axis that is contracted");
+    STD_TORCH_CHECK(a_scale.is_cuda() && a_scale.get_device_index() == device && a_scale.scalar_type() == ScalarType::Float, "a_scale must be float32 on a's device");
+    STD_TORCH_CHECK(a_scale.dim() == 2 && a_scale.size(0) == blocks_of(depth) && a_scale.size(1) == M, "a_scale must be [", blocks_of(depth), ", ", M, "]");
+    STD_TORCH_CHECK(a.is_contiguous() && a_scale.is_contiguous(), "a and a_scale must be contiguous");
+    STD_TORCH_CHECK(aligned16(a.const_data_ptr()), "a data pointer must be 16-byte aligned");
     torch::stable::accelerator::DeviceGuard guard(device);
+    Tensor c = make_empty({M, transposed_b ? K : N}, half_dtype(out_fp16), device);
     const bool ok = launch_fp8_block_mm(
         static_cast<const uint8_t*>(a.const_data_ptr()), static_cast<const float*>(a_scale.const_data_ptr()), static_cast<const uint8_t*>(weight.const_data_ptr()),
-        static_cast<const float*>(weight_scale.const_data_ptr()), bias.has_value() ? static_cast<const uint16_t*>(bias->const_data_ptr()) : nullptr,
-        static_cast<uint16_t*>(c.mutable_data_ptr()), M, N, K, transposed_b, a.scalar_type() == ScalarType::Float8_e5m2 ? 1 : 0,
-        weight.scalar_type() == ScalarType::Float8_e5m2 ? 1 : 0, c.scalar_type() == ScalarType::Half ? 0 : 1, current_stream(device));
+        static_cast<const float*>(weight_scale.const_data_ptr()), bias_ptr(bias), static_cast<uint16_t*>(c.mutable_data_ptr()), M, N, K, transposed_b,
+        a.scalar_type() == ScalarType::Float8_e5m2 ? 1 : 0, weight.scalar_type() == ScalarType::Float8_e5m2 ? 1 : 0, out_fp16 ? 0 : 1, current_stream(device));
     STD_TORCH_CHECK(ok, "fp8_block_mm launch failed");
+    return c;
+}
+
+// Quantizer and product in one call; the codes and their scales are scratch.
+Tensor fp8_block_linear(const Tensor& x, const Tensor& weight, const Tensor& weight_scale, const std::optional<Tensor>& bias, bool out_fp16, bool transposed_b,
+                        bool e5m2) {
+    check_input(x, "x", 16);
+    const auto device = x.get_device_index();
+    check_block_weight(weight, weight_scale, bias, out_fp16, transposed_b, device);
+    const int64_t M = x.size(0), N = weight.size(0), K = weight.size(1), depth = transposed_b ? N : K;
+    STD_TORCH_CHECK(x.size(1) == depth, "x's row length must equal the weight axis that is contracted");
+    torch::stable::accelerator::DeviceGuard guard(device);
+    Tensor c = make_empty({M, transposed_b ? K : N}, half_dtype(out_fp16), device);
+    Tensor scratch = make_empty({M * (depth + 4 * blocks_of(depth))}, aoti_torch_dtype_uint8(), device);   // the codes, then the scales
+    uint8_t* const q = static_cast<uint8_t*>(scratch.mutable_data_ptr());
+    const bool ok = launch_fp8_block_linear(x.const_data_ptr(), q, reinterpret_cast<float*>(q + M * depth), static_cast<const uint8_t*>(weight.const_data_ptr()),
+                                            static_cast<const float*>(weight_scale.const_data_ptr()), bias_ptr(bias),
+                                            static_cast<uint16_t*>(c.mutable_data_ptr()), M, N, K, transposed_b, is_half(x) ? 1 : 0, e5m2 ? 1 : 0,
+                                            weight.scalar_type() == ScalarType::Float8_e5m2 ? 1 : 0, out_fp16 ? 0 : 1, current_stream(device));
+    STD_TORCH_CHECK(ok, "fp8_block_linear launch failed");
+    return c;
 }
 
 // The norm's weight: [K], of the input's dtype or float32.
@@ -400,90 +452,77 @@ void check_norm_weight(const Tensor& weight, const Tensor& x, int64_t K) {
     STD_TORCH_CHECK(K <= 32768, "a norm's rows may have at most 32768 channels");
 }
 
-void rms_norm_fp8(const Tensor& x, const std::optional<Tensor>& residual, const Tensor& weight, const std::optional<Tensor>& residual_out, Tensor& q,
-                  Tensor& scale, Tensor& rstd, double eps) {
-    STD_TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
-    STD_TORCH_CHECK(is_half_or_bf16(x.scalar_type()), "x must be float16 or bfloat16");
-    STD_TORCH_CHECK(x.dim() == 2, "x must be 2D");
+std::tuple<Tensor, Tensor, Tensor> rms_norm_fp8(const Tensor& x, const std::optional<Tensor>& residual, const Tensor& weight,
+                                                std::optional<Tensor> residual_out, double eps, bool e5m2) {
+    check_input(x, "x", 16);
     const auto device = x.get_device_index();
     const int64_t M = x.size(0), K = x.size(1);
-    check_rows(x, "x", M, K, x.scalar_type(), device);
     STD_TORCH_CHECK(residual.has_value() == residual_out.has_value(), "residual and residual_out come together");
     if (residual.has_value()) {
         check_rows(*residual, "residual", M, K, x.scalar_type(), device);
         check_rows(*residual_out, "residual_out", M, K, x.scalar_type(), device);
     }
-    check_block_codes(q, scale, M, K, device);
     check_norm_weight(weight, x, K);
-    STD_TORCH_CHECK(rstd.is_cuda() && rstd.get_device_index() == device && rstd.scalar_type() == ScalarType::Float && rstd.numel() == M && rstd.is_contiguous(),
-                    "rstd must be M contiguous float32 on the input's device");
     STD_TORCH_CHECK(eps >= 0, "eps must not be negative");
     torch::stable::accelerator::DeviceGuard guard(device);
+    Tensor q = make_empty({M, K}, code_dtype(e5m2), device);
+    Tensor scale = make_empty({blocks_of(K), M}, aoti_torch_dtype_float32(), device);
+    Tensor rstd = make_empty({M}, aoti_torch_dtype_float32(), device);
     const bool ok = launch_rms_norm_fp8(x.const_data_ptr(), residual.has_value() ? residual->const_data_ptr() : nullptr, weight.const_data_ptr(),
                                         residual_out.has_value() ? residual_out->mutable_data_ptr() : nullptr, q.mutable_data_ptr(),
                                         static_cast<float*>(scale.mutable_data_ptr()), static_cast<float*>(rstd.mutable_data_ptr()), M, K, static_cast<float>(eps),
-                                        x.scalar_type() == ScalarType::Half ? 1 : 0, weight.scalar_type() == ScalarType::Float ? 1 : 0,
-                                        q.scalar_type() == ScalarType::Float8_e5m2 ? 1 : 0, current_stream(device));
+                                        is_half(x) ? 1 : 0, weight.scalar_type() == ScalarType::Float ? 1 : 0, e5m2 ? 1 : 0, current_stream(device));
     STD_TORCH_CHECK(ok, "rms_norm_fp8 launch failed");
+    return std::make_tuple(std::move(q), std::move(scale), std::move(rstd));
 }
 
-void rms_norm_dgrad(const Tensor& grad, const Tensor& x, const Tensor& weight, const Tensor& rstd, const std::optional<Tensor>& grad_residual, Tensor& grad_x,
-                    Tensor& grad_weight, Tensor& partials) {
-    STD_TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
-    STD_TORCH_CHECK(is_half_or_bf16(x.scalar_type()), "x must be float16 or bfloat16");
-    STD_TORCH_CHECK(x.dim() == 2, "x must be 2D");
+std::tuple<Tensor, Tensor> rms_norm_dgrad(const Tensor& grad, const Tensor& x, const Tensor& weight, const Tensor& rstd,
+                                          const std::optional<Tensor>& grad_residual) {
+    check_input(x, "x", 16);
     const auto device = x.get_device_index();
     const int64_t M = x.size(0), K = x.size(1);
-    STD_TORCH_CHECK(M > 0 && K > 0 && K % 16 == 0, "x must have rows, and a row length that is a positive multiple of 16");
-    check_rows(x, "x", M, K, x.scalar_type(), device);
+    STD_TORCH_CHECK(M > 0, "x must have rows");
     check_rows(grad, "grad", M, K, x.scalar_type(), device);
     if (grad_residual.has_value()) check_rows(*grad_residual, "grad_residual", M, K, x.scalar_type(), device);
-    check_rows(grad_x, "grad_x", M, K, x.scalar_type(), device);
     check_norm_weight(weight, x, K);
     STD_TORCH_CHECK(rstd.is_cuda() && rstd.get_device_index() == device && rstd.scalar_type() == ScalarType::Float && rstd.numel() == M && rstd.is_contiguous(),
                     "rstd must be M contiguous float32 on the input's device");
-    STD_TORCH_CHECK(grad_weight.is_cuda() && grad_weight.get_device_index() == device && grad_weight.scalar_type() == ScalarType::Float &&
-                        grad_weight.numel() == K && grad_weight.is_contiguous(),
-                    "grad_weight must be K contiguous float32 on the input's device");
     torch::stable::accelerator::DeviceGuard guard(device);
-    STD_TORCH_CHECK(partials.is_cuda() && partials.get_device_index() == device && partials.scalar_type() == ScalarType::Float && partials.is_contiguous() &&
-                        partials.numel() >= feather_rms_norm_dgrad_partial_floats(M, K) && aligned16(partials.const_data_ptr()),
-                    "partials must be contiguous float32 scratch of the size feather_rms_norm_dgrad_partial_floats gives");
+    Tensor grad_x = make_empty({M, K}, half_dtype(is_half(x)), device);
+    Tensor grad_weight = make_empty({K}, aoti_torch_dtype_float32(), device);
+    Tensor partials = make_empty({feather_rms_norm_dgrad_partial_floats(M, K)}, aoti_torch_dtype_float32(), device);
     const bool ok = launch_rms_norm_dgrad(grad.const_data_ptr(), x.const_data_ptr(), weight.const_data_ptr(), static_cast<const float*>(rstd.const_data_ptr()),
                                           grad_residual.has_value() ? grad_residual->const_data_ptr() : nullptr, grad_x.mutable_data_ptr(),
                                           static_cast<float*>(grad_weight.mutable_data_ptr()), static_cast<float*>(partials.mutable_data_ptr()), M, K,
-                                          x.scalar_type() == ScalarType::Half ? 1 : 0, weight.scalar_type() == ScalarType::Float ? 1 : 0, current_stream(device));
+                                          is_half(x) ? 1 : 0, weight.scalar_type() == ScalarType::Float ? 1 : 0, current_stream(device));
     STD_TORCH_CHECK(ok, "rms_norm_dgrad launch failed");
+    return std::make_tuple(std::move(grad_x), std::move(grad_weight));
 }
 
-void silu_mul_fp8(const Tensor& gate_up, Tensor& q, Tensor& scale) {
-    STD_TORCH_CHECK(gate_up.is_cuda(), "gate_up must be a CUDA tensor");
-    STD_TORCH_CHECK(is_half_or_bf16(gate_up.scalar_type()), "gate_up must be float16 or bfloat16");
-    STD_TORCH_CHECK(gate_up.dim() == 2 && gate_up.size(1) % 2 == 0, "gate_up must be [M, 2 F]");
+std::tuple<Tensor, Tensor> silu_mul_fp8(const Tensor& gate_up, bool e5m2) {
+    check_input(gate_up, "gate_up", 32);
     const auto device = gate_up.get_device_index();
     const int64_t M = gate_up.size(0), F = gate_up.size(1) / 2;
-    check_rows(gate_up, "gate_up", M, 2 * F, gate_up.scalar_type(), device);
-    check_block_codes(q, scale, M, F, device);
     torch::stable::accelerator::DeviceGuard guard(device);
+    Tensor q = make_empty({M, F}, code_dtype(e5m2), device);
+    Tensor scale = make_empty({blocks_of(F), M}, aoti_torch_dtype_float32(), device);
     const bool ok = launch_silu_mul_fp8(gate_up.const_data_ptr(), q.mutable_data_ptr(), static_cast<float*>(scale.mutable_data_ptr()), M, F,
-                                        gate_up.scalar_type() == ScalarType::Half ? 1 : 0, q.scalar_type() == ScalarType::Float8_e5m2 ? 1 : 0,
-                                        current_stream(device));
+                                        is_half(gate_up) ? 1 : 0, e5m2 ? 1 : 0, current_stream(device));
     STD_TORCH_CHECK(ok, "silu_mul_fp8 launch failed");
+    return std::make_tuple(std::move(q), std::move(scale));
 }
 
-void silu_mul_dgrad(const Tensor& grad, const Tensor& gate_up, Tensor& grad_gate_up) {
-    STD_TORCH_CHECK(gate_up.is_cuda(), "gate_up must be a CUDA tensor");
-    STD_TORCH_CHECK(is_half_or_bf16(gate_up.scalar_type()), "gate_up must be float16 or bfloat16");
-    STD_TORCH_CHECK(gate_up.dim() == 2 && gate_up.size(1) > 0 && gate_up.size(1) % 32 == 0, "gate_up must be [M, 2 F], F a positive multiple of 16");
+Tensor silu_mul_dgrad(const Tensor& grad, const Tensor& gate_up) {
+    check_input(gate_up, "gate_up", 32);
     const auto device = gate_up.get_device_index();
     const int64_t M = gate_up.size(0), F = gate_up.size(1) / 2;
-    check_rows(gate_up, "gate_up", M, 2 * F, gate_up.scalar_type(), device);
     check_rows(grad, "grad", M, F, gate_up.scalar_type(), device);
-    check_rows(grad_gate_up, "grad_gate_up", M, 2 * F, gate_up.scalar_type(), device);
     torch::stable::accelerator::DeviceGuard guard(device);
-    const bool ok = launch_silu_mul_dgrad(grad.const_data_ptr(), gate_up.const_data_ptr(), grad_gate_up.mutable_data_ptr(), M, F,
-                                          gate_up.scalar_type() == ScalarType::Half ? 1 : 0, current_stream(device));
+    Tensor out = make_empty({M, 2 * F}, half_dtype(is_half(gate_up)), device);
+    const bool ok = launch_silu_mul_dgrad(grad.const_data_ptr(), gate_up.const_data_ptr(), out.mutable_data_ptr(), M, F, is_half(gate_up) ? 1 : 0,
+                                          current_stream(device));
     STD_TORCH_CHECK(ok, "silu_mul_dgrad launch failed");
+    return out;
 }
 
 void conv2d_3x3(const Tensor& x, const Tensor& w_prepacked, const std::optional<Tensor>& bias, Tensor& out, int64_t warps_m, int64_t warps_n,
@@ -559,17 +598,15 @@ STABLE_TORCH_LIBRARY(feather_ops, m) {
         "int block_warps_m, int block_warps_n, int unroll_k, int repeat_m, int repeat_n) -> ()");
     m.def("int8_scaled_mm_plain(Tensor a, Tensor weight, Tensor a_scale, Tensor? b_scale, Tensor? bias, Tensor(a!) c, bool transposed_b) -> ()");
     m.def("convrot_quantize(Tensor x, Tensor? col_scale, Tensor(a!) q, Tensor(b!) row_scale, bool rotate) -> ()");
-    m.def("fp8_block_quantize(Tensor x, Tensor(a!) q, Tensor(b!) scale) -> ()");
+    m.def("fp8_block_quantize(Tensor x, bool e5m2) -> (Tensor, Tensor)");
     m.def(
-        "fp8_block_mm(Tensor a, Tensor a_scale, Tensor weight, Tensor weight_scale, Tensor? bias, Tensor(a!) c, bool transposed_b) -> ()");
+        "fp8_block_mm(Tensor a, Tensor a_scale, Tensor weight, Tensor weight_scale, Tensor? bias, bool out_fp16, bool transposed_b) -> Tensor");
+    m.def("fp8_block_linear(Tensor x, Tensor weight, Tensor weight_scale, Tensor? bias, bool out_fp16, bool transposed_b, bool e5m2) -> Tensor");
     m.def(
-        "rms_norm_fp8(Tensor x, Tensor? residual, Tensor weight, Tensor(a!)? residual_out, Tensor(b!) q, Tensor(c!) scale, Tensor(d!) rstd, "
-        "float eps) -> ()");
-    m.def(
-        "rms_norm_dgrad(Tensor grad, Tensor x, Tensor weight, Tensor rstd, Tensor? grad_residual, Tensor(a!) grad_x, Tensor(b!) grad_weight, "
-        "Tensor(c!) partials) -> ()");
-    m.def("silu_mul_fp8(Tensor gate_up, Tensor(a!) q, Tensor(b!) scale) -> ()");
-    m.def("silu_mul_dgrad(Tensor grad, Tensor gate_up, Tensor(a!) grad_gate_up) -> ()");
+        "rms_norm_fp8(Tensor x, Tensor? residual, Tensor weight, Tensor(a!)? residual_out, float eps, bool e5m2) -> (Tensor, Tensor, Tensor)");
+    m.def("rms_norm_dgrad(Tensor grad, Tensor x, Tensor weight, Tensor rstd, Tensor? grad_residual) -> (Tensor, Tensor)");
+    m.def("silu_mul_fp8(Tensor gate_up, bool e5m2) -> (Tensor, Tensor)");
+    m.def("silu_mul_dgrad(Tensor grad, Tensor gate_up) -> Tensor");
     m.def(
         "conv2d_3x3(Tensor x, Tensor w_prepacked, Tensor? bias, Tensor(a!) out, int warps_m, int warps_n, int repeat_m, int repeat_n, "
         "int rows, bool prefetch) -> ()");
@@ -584,6 +621,7 @@ STABLE_TORCH_LIBRARY_IMPL(feather_ops, CUDA, m) {
     m.impl("convrot_quantize", TORCH_BOX(&convrot_quantize));
     m.impl("fp8_block_quantize", TORCH_BOX(&fp8_block_quantize));
     m.impl("fp8_block_mm", TORCH_BOX(&fp8_block_mm));
+    m.impl("fp8_block_linear", TORCH_BOX(&fp8_block_linear));
     m.impl("rms_norm_fp8", TORCH_BOX(&rms_norm_fp8));
     m.impl("rms_norm_dgrad", TORCH_BOX(&rms_norm_dgrad));
     m.impl("silu_mul_fp8", TORCH_BOX(&silu_mul_fp8));

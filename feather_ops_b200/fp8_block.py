@@ -30,6 +30,7 @@ NaN. All sizes along a row are multiples of 16; matrices are contiguous and 16-b
 import torch
 
 FP8_BLOCK = 128
+_ops = torch.ops.feather_ops
 _TOP = {torch.float8_e4m3fn: 448.0, torch.float8_e5m2: 57344.0}
 _LEAST_SCALE = 1e-30  # blocks of zeros get this scale: its inverse is finite, and so is its product with a weight's scale
 
@@ -40,19 +41,25 @@ def _top(dtype: torch.dtype) -> float:
     return _TOP[dtype]
 
 
+def _is_e5m2(dtype: torch.dtype) -> bool:
+    if dtype is torch.float8_e4m3fn:
+        return False
+    _top(dtype)
+    return True
+
+
+def _is_fp16(dtype: torch.dtype) -> bool:
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
+        raise ValueError(f"the output must be float16 or bfloat16, got {dtype}")
+    return dtype is torch.float16
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    return x if x.ndim == 2 else x.reshape(-1, x.shape[-1])
+
+
 def _blocks(size: int) -> int:
     return -(-size // FP8_BLOCK)
-
-
-def _norm_partials(rows: int, width: int) -> int:
-    """Floats of scratch for the norm's weight gradient (the rule of `feather_rms_norm_dgrad_partial_floats`)."""
-    return min(-(-rows // 4), 296) * width
-
-
-def _empty_codes(rows: int, width: int, dtype: torch.dtype, device) -> tuple[torch.Tensor, torch.Tensor]:
-    _top(dtype)
-    q = torch.empty((rows, width), device=device, dtype=dtype)
-    return q, torch.empty((_blocks(width), rows), device=device, dtype=torch.float32)
 
 
 def quantize_fp8_weight(weight: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> tuple[torch.Tensor, torch.Tensor]:
@@ -80,38 +87,36 @@ def dequantize_fp8_weight(q: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
 def quantize_fp8_activation(x: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> tuple[torch.Tensor, torch.Tensor]:
     """Codes and block scales of a `[M, K]` fp16/bf16 activation, in one kernel: with `t` the largest magnitude of a block
     (at least `1e-30 * top`), `scale = t / top` and `q = fp8(x * (top / t))`. Returns `(q [M, K], scale [ceil(K / 128), M])`."""
-    q, scale = _empty_codes(x.shape[0], x.shape[1], dtype, x.device)
-    torch.ops.feather_ops.fp8_block_quantize.default(x, q, scale)
-    return q, scale
+    return _ops.fp8_block_quantize.default(x, _is_e5m2(dtype))
 
 
 def fp8_block_mm(a, a_scale, weight, weight_scale, bias=None, out_dtype=torch.bfloat16, transposed_b=False):
     """`A @ W^T + bias` (or `A @ W` with `transposed_b`) of fp8 codes with block scales, accumulated in float32 and rounded
     once. `a` `[M, K]` (`[M, N]`) with `a_scale` as `quantize_fp8_activation` gives them; `weight` `[N, K]` with
     `weight_scale`. Either side may be e4m3 or e5m2. `bias` (forward only) has `N` values of `out_dtype`."""
-    n, k = weight.shape
-    out = torch.empty((a.shape[0], k if transposed_b else n), device=a.device, dtype=out_dtype)
-    torch.ops.feather_ops.fp8_block_mm.default(a, a_scale, weight, weight_scale, bias, out, transposed_b)
-    return out
+    return _ops.fp8_block_mm.default(a, a_scale, weight, weight_scale, bias, _is_fp16(out_dtype), transposed_b)
+
+
+def _quantized_product(x, weight, weight_scale, bias, out_dtype, dtype, transposed_b):
+    """Quantizer and product of `x` `[..., depth]`, two launches of one operator call."""
+    out = _ops.fp8_block_linear.default(_rows(x), weight, weight_scale, bias, _is_fp16(out_dtype), transposed_b, _is_e5m2(dtype))
+    return out if x.ndim == 2 else out.view(*x.shape[:-1], out.shape[1])
 
 
 def fp8_block_linear(x, weight, weight_scale, bias=None, out_dtype=torch.bfloat16, dtype=torch.float8_e4m3fn):
-    """Forward `x @ W^T + bias` of a 16-bit activation `[..., K]`: quantized to `dtype`, then the product."""
-    n, k = weight.shape
-    if x.shape[-1] != k:
-        raise ValueError(f"activation has {x.shape[-1]} features, the weight {k}")
-    q, scale = quantize_fp8_activation(x.reshape(-1, k), dtype)
-    return fp8_block_mm(q, scale, weight, weight_scale, bias, out_dtype).reshape(*x.shape[:-1], n)
+    """Forward `x @ W^T + bias` of a 16-bit activation `[..., K]`: quantized to `dtype`, then the product. The bits are those of
+    `quantize_fp8_activation` and `fp8_block_mm`."""
+    if x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"activation has {x.shape[-1]} features, the weight {weight.shape[1]}")
+    return _quantized_product(x, weight, weight_scale, bias, out_dtype, dtype, False)
 
 
 def fp8_block_dgrad(grad_out, weight, weight_scale, out_dtype=torch.bfloat16, dtype=torch.float8_e4m3fn):
     """Input gradient `g @ W` of a 16-bit `[..., N]` gradient, quantized to `dtype` along its own rows: the weight's codes and
     block scales are those of the forward product."""
-    n, k = weight.shape
-    if grad_out.shape[-1] != n:
-        raise ValueError(f"gradient has {grad_out.shape[-1]} features, the weight {n}")
-    q, scale = quantize_fp8_activation(grad_out.reshape(-1, n), dtype)
-    return fp8_block_mm(q, scale, weight, weight_scale, None, out_dtype, True).reshape(*grad_out.shape[:-1], k)
+    if grad_out.shape[-1] != weight.shape[0]:
+        raise ValueError(f"gradient has {grad_out.shape[-1]} features, the weight {weight.shape[0]}")
+    return _quantized_product(grad_out, weight, weight_scale, None, out_dtype, dtype, True)
 
 
 def rms_norm_quantize_fp8(x, weight, residual=None, eps=1e-6, dtype=torch.float8_e4m3fn):
@@ -121,46 +126,33 @@ def rms_norm_quantize_fp8(x, weight, residual=None, eps=1e-6, dtype=torch.float8
 
     Returns `(q [rows, K], scale [ceil(K / 128), rows], h, rstd [rows])`: `h` has x's shape and is x itself without a residual;
     `rstd` is what the backward pass needs."""
-    k = x.shape[-1]
     if residual is not None and residual.shape != x.shape:
         raise ValueError(f"residual is {tuple(residual.shape)}, x {tuple(x.shape)}")
-    rows = x.reshape(-1, k)
-    q, scale = _empty_codes(rows.shape[0], k, dtype, x.device)
-    rstd = torch.empty(rows.shape[0], device=x.device, dtype=torch.float32)
+    rows = _rows(x)
     if residual is None:
-        torch.ops.feather_ops.rms_norm_fp8.default(rows, None, weight, None, q, scale, rstd, eps)
+        q, scale, rstd = _ops.rms_norm_fp8.default(rows, None, weight, None, eps, _is_e5m2(dtype))
         return q, scale, x, rstd
     stream = torch.empty_like(rows)
-    torch.ops.feather_ops.rms_norm_fp8.default(rows, residual.reshape(-1, k), weight, stream, q, scale, rstd, eps)
-    return q, scale, stream.view(x.shape), rstd
+    q, scale, rstd = _ops.rms_norm_fp8.default(rows, _rows(residual), weight, stream, eps, _is_e5m2(dtype))
+    return q, scale, stream.view(x.shape) if x.ndim != 2 else stream, rstd
 
 
 def rms_norm_dgrad(grad_out, x, weight, rstd, grad_residual=None):
     """Backward pass of the norm: `x` is what it was taken of (`h` of `rms_norm_quantize_fp8`), `grad_out` the gradient of
     its output. `grad_residual`, the gradient that reaches `h` along the residual stream, is added in the same pass; the result
     is the gradient of both `x` and the residual of the forward call. Returns `(grad_x, grad_weight float32 [K])`."""
-    k = x.shape[-1]
     if grad_out.shape != x.shape or (grad_residual is not None and grad_residual.shape != x.shape):
         raise ValueError("grad_out and grad_residual must have x's shape")
-    rows = x.reshape(-1, k)
-    m = rows.shape[0]
-    grad_x = torch.empty_like(rows)
-    if m == 0:
-        return grad_x.view(x.shape), torch.zeros(k, device=x.device, dtype=torch.float32)
-    grad_weight = torch.empty(k, device=x.device, dtype=torch.float32)
-    partials = torch.empty(_norm_partials(m, k), device=x.device, dtype=torch.float32)
-    residual = None if grad_residual is None else grad_residual.reshape(-1, k)
-    torch.ops.feather_ops.rms_norm_dgrad.default(grad_out.reshape(-1, k), rows, weight, rstd, residual, grad_x, grad_weight, partials)
-    return grad_x.view(x.shape), grad_weight
+    if x.numel() == 0:
+        return torch.empty_like(x), torch.zeros(x.shape[-1], device=x.device, dtype=torch.float32)
+    grad_x, grad_weight = _ops.rms_norm_dgrad.default(_rows(grad_out), _rows(x), weight, rstd, None if grad_residual is None else _rows(grad_residual))
+    return grad_x if x.ndim == 2 else grad_x.view(x.shape), grad_weight
 
 
 def silu_mul_quantize_fp8(gate_up, dtype=torch.float8_e4m3fn):
     """Codes and block scales of `silu(gate) * up`, in one kernel. `gate_up` `[..., 2 F]` fp16/bf16 with the gate's columns
     first. Returns `(q [rows, F], scale [ceil(F / 128), rows])`."""
-    rows = gate_up.reshape(-1, gate_up.shape[-1])
-    q, scale = _empty_codes(rows.shape[0], rows.shape[1] // 2, dtype, gate_up.device)
-    torch.ops.feather_ops.silu_mul_fp8.default(rows, q, scale)
-    return q, scale
+    return _ops.silu_mul_fp8.default(_rows(gate_up), _is_e5m2(dtype))
 
 
 def silu_mul_dgrad(grad_out, gate_up):
@@ -168,12 +160,50 @@ def silu_mul_dgrad(grad_out, gate_up):
     f = gate_up.shape[-1] // 2
     if grad_out.shape != (*gate_up.shape[:-1], f):
         raise ValueError(f"grad_out is {tuple(grad_out.shape)}, gate_up {tuple(gate_up.shape)}")
-    rows = gate_up.reshape(-1, gate_up.shape[-1])
-    out = torch.empty_like(rows)
-    torch.ops.feather_ops.silu_mul_dgrad.default(grad_out.reshape(-1, f), rows, out)
-    return out.view(gate_up.shape)
+    out = _ops.silu_mul_dgrad.default(_rows(grad_out), _rows(gate_up))
+    return out if gate_up.ndim == 2 else out.view(gate_up.shape)
 
 
-for _name in ("fp8_block_quantize", "fp8_block_mm", "rms_norm_fp8", "rms_norm_dgrad", "silu_mul_fp8", "silu_mul_dgrad"):
-    # every operator writes into its arguments and returns nothing, which is all that a compiled caller has to know
-    torch.library.register_fake(f"feather_ops::{_name}", lambda *args: None)
+# What a compiled caller has to know of the operators: the shapes and types of what they return.
+def _fake_codes(rows, width, like, e5m2):
+    dtype = torch.float8_e5m2 if e5m2 else torch.float8_e4m3fn
+    return like.new_empty((rows, width), dtype=dtype), like.new_empty((_blocks(width), rows), dtype=torch.float32)
+
+
+def _fake_out(rows, weight, like, out_fp16, transposed_b):
+    return like.new_empty((rows, weight.shape[1 if transposed_b else 0]), dtype=torch.float16 if out_fp16 else torch.bfloat16)
+
+
+@torch.library.register_fake("feather_ops::fp8_block_quantize")
+def _(x, e5m2):
+    return _fake_codes(x.shape[0], x.shape[1], x, e5m2)
+
+
+@torch.library.register_fake("feather_ops::fp8_block_mm")
+def _(a, a_scale, weight, weight_scale, bias, out_fp16, transposed_b):
+    return _fake_out(a.shape[0], weight, a, out_fp16, transposed_b)
+
+
+@torch.library.register_fake("feather_ops::fp8_block_linear")
+def _(x, weight, weight_scale, bias, out_fp16, transposed_b, e5m2):
+    return _fake_out(x.shape[0], weight, x, out_fp16, transposed_b)
+
+
+@torch.library.register_fake("feather_ops::rms_norm_fp8")
+def _(x, residual, weight, residual_out, eps, e5m2):
+    return *_fake_codes(x.shape[0], x.shape[1], x, e5m2), x.new_empty((x.shape[0],), dtype=torch.float32)
+
+
+@torch.library.register_fake("feather_ops::rms_norm_dgrad")
+def _(grad, x, weight, rstd, grad_residual):
+    return torch.empty_like(x), x.new_empty((x.shape[1],), dtype=torch.float32)
+
+
+@torch.library.register_fake("feather_ops::silu_mul_fp8")
+def _(gate_up, e5m2):
+    return _fake_codes(gate_up.shape[0], gate_up.shape[1] // 2, gate_up, e5m2)
+
+
+@torch.library.register_fake("feather_ops::silu_mul_dgrad")
+def _(grad, gate_up):
+    return torch.empty_like(gate_up)

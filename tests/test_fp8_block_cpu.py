@@ -4,7 +4,6 @@ import pytest
 import torch
 
 import feather_ops_b200 as fo
-from feather_ops_b200 import fp8_block
 from oracle import fp8_block as ofb
 
 E4M3, E5M2 = torch.float8_e4m3fn, torch.float8_e5m2
@@ -47,6 +46,8 @@ def test_calls_that_are_refused_before_any_kernel():
         fo.fp8_block_dgrad(x, w, scale)
     with pytest.raises(ValueError, match="float8"):
         fo.quantize_fp8_activation(x, torch.int8)
+    with pytest.raises(ValueError, match="output"):
+        fo.fp8_block_mm(x.to(E4M3), torch.ones(1, 4), w, scale, None, torch.float32)
     with pytest.raises(ValueError, match="residual"):
         fo.rms_norm_quantize_fp8(x, torch.ones(128), x[:2])
     with pytest.raises(ValueError, match="shape"):
@@ -80,9 +81,10 @@ def test_launchers_refuse_bad_arguments_without_a_device(lib):
     assert not lib.launch_silu_mul_dgrad(p, p, None, 4, 16, 0, None)
 
 
-@pytest.mark.parametrize("m", [1, 3, 4, 5, 1183, 1184, 1185, 8192])
-def test_scratch_size_is_the_librarys(lib, m):
-    assert fp8_block._norm_partials(m, 272) == lib.feather_rms_norm_dgrad_partial_floats(m, 272)
+def test_scratch_of_the_norms_weight_gradient(lib):
+    # four rows per CTA at least, 296 CTAs at most
+    for m, ctas in ((0, 0), (1, 1), (4, 1), (5, 2), (1184, 296), (1185, 296), (100000, 296)):
+        assert lib.feather_rms_norm_dgrad_partial_floats(m, 272) == ctas * 272
 
 
 def test_norm_gradient_formula_against_differences():

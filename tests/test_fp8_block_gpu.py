@@ -130,7 +130,7 @@ def test_product_keeps_rows_apart_and_the_memory_around_them(cuda_device, m, tra
     out = room[2 * width : (m + 2) * width].view(m, width)
     s_bad = s.clone()
     s_bad[1, 1] = float("nan")
-    torch.ops.feather_ops.fp8_block_mm.default(q, s_bad, w, ws, None, out, transposed)
+    assert _lib.load().launch_fp8_block_mm(q.data_ptr(), s_bad.data_ptr(), w.data_ptr(), ws.data_ptr(), None, out.data_ptr(), m, n, k, transposed, 0, 0, 1, torch.cuda.current_stream().cuda_stream)
     assert out[1].isnan().all()
     keep = [r for r in range(m) if r != 1]
     assert torch.equal(out[keep], clean[keep])
