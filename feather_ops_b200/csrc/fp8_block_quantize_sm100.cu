@@ -2,17 +2,18 @@
 // silu(gate) * up with their outputs in 8 bits, and the backward passes of the last two.
 //
 // Block scales. Every 128 consecutive channels of a row share one float32 scale:
-//     t = max(max |y|, 1e-30 * top),  scale = t / top,  code = fp8(y * (top / t)),  top = 448 (e4m3) or 57344 (e5m2).
-// One division per block and one product per element; the floor on t keeps the inverse finite for blocks of zeros. The
-// maximum is taken on the bit patterns of |y|, where a NaN is larger than any number, so a block that holds an infinity
-// or a NaN gets a scale that is not finite and never reads back as ordinary numbers.
-// The scales are laid out [ceil(K / 128), M]: the product's epilogue wants the scales of consecutive rows at one block.
+//     t = max(max |y|, 1e-30 * top),  scale = t * (1 / top),  code = fp8(y * (top * (1 / t))),  top = 448 (e4m3) or 57344 (e5m2).
+// One reciprocal per block and one product per element; the floor on t keeps the inverse finite for blocks of zeros. The maximum
+// keeps NaN, so a block that holds an infinity or a NaN never reads back as ordinary numbers.
+// The scales are laid out [ceil(K / 128), M]: the product wants the scales of consecutive rows at one block.
 //
-// Every kernel may start while the one ahead in its stream ends (programmatic dependent launch), waits for it before it
-// reads or writes memory, and lets the next one start likewise.
+// Every kernel but the norm's backward pass may start while the one ahead in its stream ends (programmatic dependent launch),
+// waits for it before it reads or writes memory, and lets the next one start likewise.
 //
-// All five kernels are bound by HBM: a thread moves 8 consecutive channels (one 16-byte load, one 8-byte store of codes),
-// 16 lanes hold one block, and its maximum is four shuffles.
+// All kernels move a few bytes per element through HBM, so few instructions per element are left: at 6.5 TB/s an SM gets 4 to 13
+// elements per clock and issues 4 warp instructions, i.e. 10 to 30 instructions per element. A thread has 8 consecutive channels
+// (one 16-byte load, one 8-byte store of codes) as four float pairs for the packed fp32 arithmetic; 16 lanes hold one block, and
+// its maximum is four shuffles.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -39,56 +40,86 @@ struct Code {
     static constexpr float kLeast = static_cast<float>(1e-30 * static_cast<double>(kTop));
 };
 
+using Pairs = float2[kVec / 2];   // 8 channels
+
 template <bool kFp16>
-__device__ __forceinline__ void unpack8(const uint4& p, float (&v)[kVec]) {
+__device__ __forceinline__ void unpack8(const uint4& p, Pairs& v) {
     const uint32_t w[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if constexpr (kFp16) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-            v[2 * i] = f.x;
-            v[2 * i + 1] = f.y;
+            v[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
         } else {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
         }
     }
 }
 
 template <bool kFp16>
-__device__ __forceinline__ uint4 pack8(const float (&v)[kVec]) {
+__device__ __forceinline__ uint4 pack8(const Pairs& v) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if constexpr (kFp16) {
-            const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+            const __half2 h = __float22half2_rn(v[i]);
             w[i] = *reinterpret_cast<const uint32_t*>(&h);
         } else {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            const __nv_bfloat162 h = __float22bfloat162_rn(v[i]);
             w[i] = *reinterpret_cast<const uint32_t*>(&h);
         }
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// The 16 lanes of a block agree on its maximum (as the bits of |y|) and turn their values into codes. Every lane of the
-// warp takes part; lanes past the row's end bring zeros.
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// max(a, |b|, |c|), NaN if any of them is
+__device__ __forceinline__ float max_magnitude(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(fabsf(b)), "f"(fabsf(c)));
+    return d;
+}
+
+__device__ __forceinline__ float max_magnitude(const Pairs& v) {
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = max_magnitude(top, v[i].x, v[i].y);
+    return top;
+}
+
+// The largest magnitude of 8 packed 16-bit values; the comparison is exact in their own type.
+template <bool kFp16>
+__device__ __forceinline__ float max_magnitude_packed(const uint4& p) {
+    const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+    if constexpr (kFp16) {
+        __half2 top = __habs2(*reinterpret_cast<const __half2*>(&w[0]));
+#pragma unroll
+        for (int i = 1; i < 4; ++i) top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __half2*>(&w[i])));
+        return __half2float(__hmax_nan(__low2half(top), __high2half(top)));
+    } else {
+        __nv_bfloat162 top = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[0]));
+#pragma unroll
+        for (int i = 1; i < 4; ++i) top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[i])));
+        return __bfloat162float(__hmax_nan(__low2bfloat16(top), __high2bfloat16(top)));
+    }
+}
+
+// The 16 lanes of a block agree on its maximum and turn their values into codes. Every lane of the warp takes part; lanes past
+// the row's end bring zeros.
 template <bool kE5M2>
-__device__ __forceinline__ uint2 encode_block(const float (&v)[kVec], float& scale) {
-    uint32_t top = 0;
+__device__ __forceinline__ uint2 encode_block(const Pairs& v, float top, float& scale) {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-#pragma unroll
-    for (int step = 8; step > 0; step >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, step));
-    const float t = __uint_as_float(max(top, __float_as_uint(Code<kE5M2>::kLeast)));
-    const float inverse = Code<kE5M2>::kTop / t;
-    scale = t / Code<kE5M2>::kTop;
+    for (int step = 8; step > 0; step >>= 1) {
+        const float other = __shfl_xor_sync(0xffffffffu, top, step);
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(other));
+    }
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(Code<kE5M2>::kLeast));
+    const float2 inverse = both(Code<kE5M2>::kTop * __frcp_rn(top));
+    scale = top * (1.0f / Code<kE5M2>::kTop);
     constexpr __nv_fp8_interpretation_t kind = kE5M2 ? __NV_E5M2 : __NV_E4M3;
     uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        w[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i] * inverse, v[2 * i + 1] * inverse), __NV_SATFINITE, kind);
-    }
+    for (int i = 0; i < 4; ++i) w[i] = __nv_cvt_float2_to_fp8x2(__fmul2_rn(v[i], inverse), __NV_SATFINITE, kind);
     return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
 }
 
@@ -100,7 +131,17 @@ __device__ __forceinline__ void start_after_kernel_ahead() {
 
 __device__ __forceinline__ uint4 load16(const uint16_t* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
 
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
+// 1 / (1 + exp(-x)), each of the two special functions once
+__device__ __forceinline__ float2 sigmoid(float2 x) {
+    const float2 e = __fmul2_rn(x, both(-1.44269504f));   // -log2(e) x
+    float2 d;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d.x) : "f"(e.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d.y) : "f"(e.y));
+    d = __fadd2_rn(d, both(1.0f));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(d.x));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(d.y));
+    return d;
+}
 
 // ---------------------------------------------------------------------------------------------------------
 // Activation quantizer and the gate: a warp takes 256 channels of kRows rows, so a thread has kRows (or 2 * kRows)
@@ -129,16 +170,19 @@ __global__ void __launch_bounds__(32 * kTileWarps) tile_quantize_kernel(const ui
     }
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-        float v[kVec];
+        Pairs v;
         unpack8<kFp16>(a[r], v);
+        float s;
+        uint2 codes;
         if constexpr (kGate) {
-            float up[kVec];
+            Pairs up;
             unpack8<kFp16>(b[r], up);
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) v[i] = v[i] * sigmoid(v[i]) * up[i];
+            for (int i = 0; i < 4; ++i) v[i] = __fmul2_rn(__fmul2_rn(v[i], sigmoid(v[i])), up[i]);
+            codes = encode_block<kE5M2>(v, max_magnitude(v), s);
+        } else {
+            codes = encode_block<kE5M2>(v, max_magnitude_packed<kFp16>(a[r]), s);
         }
-        float s;
-        const uint2 codes = encode_block<kE5M2>(v, s);
         if (live && row0 + r < M) {
             *reinterpret_cast<uint2*>(q + (row0 + r) * K + column) = codes;
             if ((lane & 15) == 0) scale[column / kBlock * M + row0 + r] = s;
@@ -160,16 +204,17 @@ __global__ void __launch_bounds__(256) silu_mul_dgrad_kernel(const uint16_t* __r
     const uint4 pg = load16(grad + row * F + column);
     const uint4 pa = load16(gate_up + at);
     const uint4 pu = load16(gate_up + at + F);
-    float g[kVec], gate[kVec], up[kVec];
+    Pairs g, gate, up;
     unpack8<kFp16>(pg, g);
     unpack8<kFp16>(pa, gate);
     unpack8<kFp16>(pu, up);
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-        const float s = sigmoid(gate[i]);
-        const float gs = g[i] * s;
-        const float d_up = gs * gate[i];
-        gate[i] = gs * up[i] * (1.0f + gate[i] * (1.0f - s));
+    for (int i = 0; i < 4; ++i) {
+        const float2 s = sigmoid(gate[i]);
+        const float2 gs = __fmul2_rn(g[i], s);
+        const float2 d_up = __fmul2_rn(gs, gate[i]);
+        const float2 rest = __ffma2_rn(s, both(-1.0f), both(1.0f));   // 1 - s
+        gate[i] = __fmul2_rn(__fmul2_rn(gs, up[i]), __ffma2_rn(gate[i], rest, both(1.0f)));
         up[i] = d_up;
     }
     *reinterpret_cast<uint4*>(out + at) = pack8<kFp16>(gate);
@@ -177,17 +222,20 @@ __global__ void __launch_bounds__(256) silu_mul_dgrad_kernel(const uint16_t* __r
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// RMS norm: one row per CTA, the row stays in registers (packed, it is 16-bit data) between the two passes.
+// RMS norm. A row belongs to blockDim.x threads: one warp up to 1024 channels (blockDim.y rows per CTA, no barrier), else
+// the whole CTA. Between the two passes it stays in registers, packed (it is 16-bit data).
 // ---------------------------------------------------------------------------------------------------------
-// Sum over the CTA in a fixed order, the same value in every thread. `slots` holds one float per warp; two barriers, so
-// the caller may come back at once with the same slots.
-__device__ __forceinline__ float block_sum(float v, float* slots) {
+constexpr int kWarpRowWidth = 1024;   // a row of at most this many channels is one warp's
+constexpr int kRowsPerCta = 8;        // ... with so many of them in a CTA
+
+// Sum over the row's threads in a fixed order, the same value in every thread. `slots`: 32 floats that nobody else uses until the
+// next barrier after this call's.
+__device__ __forceinline__ float row_sum(float v, float* slots) {
 #pragma unroll
     for (int step = 16; step > 0; step >>= 1) v += __shfl_xor_sync(0xffffffffu, v, step);
     const int warps = blockDim.x >> 5;
     if (warps == 1) return v;
     const int lane = threadIdx.x & 31;
-    __syncthreads();
     if (lane == 0) slots[threadIdx.x >> 5] = v;
     __syncthreads();
     v = lane < warps ? slots[lane] : 0.0f;
@@ -197,12 +245,12 @@ __device__ __forceinline__ float block_sum(float v, float* slots) {
 }
 
 template <bool kFp16, bool kWeightF32>
-__device__ __forceinline__ void load_weight(const void* weight, int64_t column, float (&w)[kVec]) {
+__device__ __forceinline__ void load_weight(const void* weight, int64_t column, Pairs& w) {
     if constexpr (kWeightF32) {
         const float4* const p = reinterpret_cast<const float4*>(static_cast<const float*>(weight) + column);
         const float4 lo = __ldg(p), hi = __ldg(p + 1);
-        w[0] = lo.x, w[1] = lo.y, w[2] = lo.z, w[3] = lo.w;
-        w[4] = hi.x, w[5] = hi.y, w[6] = hi.z, w[7] = hi.w;
+        w[0] = make_float2(lo.x, lo.y), w[1] = make_float2(lo.z, lo.w);
+        w[2] = make_float2(hi.x, hi.y), w[3] = make_float2(hi.z, hi.w);
     } else {
         unpack8<kFp16>(load16(static_cast<const uint16_t*>(weight) + column), w);
     }
@@ -220,65 +268,87 @@ struct NormParams {
     float eps;
 };
 
-template <bool kFp16, bool kWeightF32, bool kE5M2, int kChunks>
+// kRows rows at a time, so that without a residual there are as many loads in flight as with one.
+template <bool kFp16, bool kWeightF32, bool kE5M2, int kChunks, int kRows>
 __global__ void __launch_bounds__(kMaxNormThreads) rms_norm_fp8_kernel(const NormParams p) {
-    __shared__ float slots[32];
+    __shared__ float slots[kRows * 32];
     start_after_kernel_ahead();
-    const int64_t row = blockIdx.x;
-    const int64_t base = row * p.K;
+    const int64_t row0 = (static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y) * kRows;
+    if (row0 >= p.M) return;   // a whole warp, and with more than one warp per row the whole CTA
+    const int column0 = threadIdx.x * kVec;
     const int step = blockDim.x * kVec;
-    const int lane = threadIdx.x & 31;
-    uint4 h[kChunks];
+    const int width = static_cast<int>(p.K);
+    uint4 h[kRows][kChunks];
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-        const int64_t column = threadIdx.x * kVec + c * step;
-        h[c] = column < p.K ? load16(p.x + base + column) : make_uint4(0, 0, 0, 0);
+    for (int r = 0; r < kRows; ++r) {
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+            const bool live = column0 + c * step < width && row0 + r < p.M;
+            h[r][c] = live ? load16(p.x + (row0 + r) * p.K + column0 + c * step) : make_uint4(0, 0, 0, 0);
+        }
     }
     if (p.residual != nullptr) {
-        uint4 r[kChunks];
+        uint4 add[kRows][kChunks];
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-            const int64_t column = threadIdx.x * kVec + c * step;
-            r[c] = column < p.K ? load16(p.residual + base + column) : make_uint4(0, 0, 0, 0);
+        for (int r = 0; r < kRows; ++r) {
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+                const bool live = column0 + c * step < width && row0 + r < p.M;
+                add[r][c] = live ? load16(p.residual + (row0 + r) * p.K + column0 + c * step) : make_uint4(0, 0, 0, 0);
+            }
         }
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-            const int64_t column = threadIdx.x * kVec + c * step;
-            float a[kVec], b[kVec];
-            unpack8<kFp16>(h[c], a);
-            unpack8<kFp16>(r[c], b);
+        for (int r = 0; r < kRows; ++r) {
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) a[i] += b[i];
-            h[c] = pack8<kFp16>(a);  // the stream is kept in 16 bits, and the norm is taken of what is kept
-            if (column < p.K) *reinterpret_cast<uint4*>(p.stream + base + column) = h[c];
+            for (int c = 0; c < kChunks; ++c) {
+                Pairs a, b;
+                unpack8<kFp16>(h[r][c], a);
+                unpack8<kFp16>(add[r][c], b);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) a[i] = __fadd2_rn(a[i], b[i]);
+                h[r][c] = pack8<kFp16>(a);  // the stream is kept in 16 bits, and the norm is taken of what is kept
+                if (column0 + c * step < width && row0 + r < p.M) *reinterpret_cast<uint4*>(p.stream + (row0 + r) * p.K + column0 + c * step) = h[r][c];
+            }
         }
     }
-    float squares = 0.0f;
+    float sum[kRows];
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-        float v[kVec];
-        unpack8<kFp16>(h[c], v);
+    for (int r = 0; r < kRows; ++r) {
+        float2 squares = both(0.0f);
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) squares = fmaf(v[i], v[i], squares);
-    }
-    const float rstd = rsqrtf(block_sum(squares, slots) / static_cast<float>(p.K) + p.eps);
-    if (threadIdx.x == 0) p.rstd[row] = rstd;
+        for (int c = 0; c < kChunks; ++c) {
+            Pairs v;
+            unpack8<kFp16>(h[r][c], v);
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-        const int64_t column = threadIdx.x * kVec + c * step;
-        const bool live = column < p.K;
-        float v[kVec], w[kVec];
-        unpack8<kFp16>(h[c], v);
-        if (live) {
-            load_weight<kFp16, kWeightF32>(p.weight, column, w);
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) v[i] = v[i] * rstd * w[i];
+            for (int i = 0; i < 4; ++i) squares = __ffma2_rn(v[i], v[i], squares);
         }
-        float s;
-        const uint2 codes = encode_block<kE5M2>(v, s);
-        if (live) {
-            *reinterpret_cast<uint2*>(p.q + base + column) = codes;
-            if ((lane & 15) == 0) p.scale[column / kBlock * p.M + row] = s;
+        sum[r] = squares.x + squares.y;
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) sum[r] = row_sum(sum[r], slots + r * 32);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        sum[r] = rsqrtf(sum[r] / static_cast<float>(width) + p.eps);
+        if (threadIdx.x == 0 && row0 + r < p.M) p.rstd[row0 + r] = sum[r];
+    }
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+        const int column = column0 + c * step;
+        const bool live = column < width;
+        Pairs w = {};
+        if (live) load_weight<kFp16, kWeightF32>(p.weight, column, w);
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+            Pairs v;
+            unpack8<kFp16>(h[r][c], v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = __fmul2_rn(__fmul2_rn(v[i], both(sum[r])), w[i]);
+            float s;
+            const uint2 codes = encode_block<kE5M2>(v, max_magnitude(v), s);
+            if (live && row0 + r < p.M) {
+                *reinterpret_cast<uint2*>(p.q + (row0 + r) * p.K + column) = codes;
+                if ((threadIdx.x & 15) == 0) p.scale[column / kBlock * p.M + row0 + r] = s;
+            }
         }
     }
 }
@@ -295,74 +365,103 @@ struct NormGradParams {
 };
 
 // n = x rstd, u = grad w:  dx = rstd (u - n mean(u n)) + grad_residual,  dw = sum over rows of grad n.
-// A CTA walks rows blockIdx.x, + gridDim.x, ... and keeps its share of dw in registers, so that dw costs one row of
-// partials per CTA; a second kernel adds those in CTA order (the same bits on every run).
-template <bool kFp16, bool kWeightF32, int kChunks>
-__global__ void __launch_bounds__(kMaxNormThreads) rms_norm_dgrad_kernel(const NormGradParams p) {
-    __shared__ float slots[32];
-    start_after_kernel_ahead();
+// A persistent grid: every CTA walks its rows and keeps its share of dw in registers, so that dw costs one row of partials per
+// CTA; a second kernel adds those in CTA order (the same bits on every run). A row is a chain of latencies (loads, ten shuffles, a
+// barrier), so what counts is how many rows an SM has at once: at 64 registers four CTAs of 256 threads. (Copying the next rows to
+// shared memory ahead of time was slower at the two or three CTAs that fit then: 68 to 75 us at 8192 x 4096 with a residual.)
+template <bool kFp16, bool kWeightF32, int kChunks, int kThreads>
+__global__ void __launch_bounds__(kThreads) rms_norm_dgrad_kernel(const NormGradParams p) {
+    __shared__ float slots[2][32];
+    extern __shared__ float total[];   // the width, with several rows per CTA
+    const int column0 = threadIdx.x * kVec;
     const int step = blockDim.x * kVec;
-    float dw[kChunks][kVec];
+    const int width = static_cast<int>(p.K);
+    const int64_t row_step = static_cast<int64_t>(gridDim.x) * blockDim.y;
+    float2 dw[kChunks][4];
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) dw[c][i] = 0.0f;
+        for (int i = 0; i < 4; ++i) dw[c][i] = both(0.0f);
     }
-    for (int64_t row = blockIdx.x; row < p.M; row += gridDim.x) {
+    bool odd = false;
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; row < p.M; row += row_step) {
         const int64_t base = row * p.K;
         const float rstd = __ldg(p.rstd + row);
-        uint4 x[kChunks], g[kChunks], r[kChunks];
+        uint4 x[kChunks], g[kChunks], res[kChunks];
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
-            const int64_t column = threadIdx.x * kVec + c * step;
-            const bool live = column < p.K;
-            x[c] = live ? load16(p.x + base + column) : make_uint4(0, 0, 0, 0);
-            g[c] = live ? load16(p.grad + base + column) : make_uint4(0, 0, 0, 0);
-            r[c] = live && p.grad_residual != nullptr ? load16(p.grad_residual + base + column) : make_uint4(0, 0, 0, 0);
+            const int column = column0 + c * step;
+            x[c] = g[c] = res[c] = make_uint4(0, 0, 0, 0);
+            if (column < width) {
+                x[c] = load16(p.x + base + column);
+                g[c] = load16(p.grad + base + column);
+                if (p.grad_residual != nullptr) res[c] = load16(p.grad_residual + base + column);
+            }
         }
-        float dot = 0.0f;
+        float2 dots = both(0.0f);
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
-            const int64_t column = threadIdx.x * kVec + c * step;
-            if (column < p.K) {
-                float n[kVec], u[kVec], w[kVec];
+            const int column = column0 + c * step;
+            if (column < width) {
+                Pairs n, u, w;
                 unpack8<kFp16>(x[c], n);
                 unpack8<kFp16>(g[c], u);
                 load_weight<kFp16, kWeightF32>(p.weight, column, w);
 #pragma unroll
-                for (int i = 0; i < kVec; ++i) {
-                    n[i] *= rstd;
-                    dw[c][i] = fmaf(u[i], n[i], dw[c][i]);
-                    dot = fmaf(u[i] * w[i], n[i], dot);
+                for (int i = 0; i < 4; ++i) {
+                    n[i] = __fmul2_rn(n[i], both(rstd));
+                    dw[c][i] = __ffma2_rn(u[i], n[i], dw[c][i]);
+                    dots = __ffma2_rn(__fmul2_rn(u[i], w[i]), n[i], dots);
                 }
             }
         }
-        const float mean = block_sum(dot, slots) / static_cast<float>(p.K);
+        const float dot = row_sum(dots.x + dots.y, slots[odd ? 1 : 0]);   // two sets of slots: a thread may still read the other one
+        odd = !odd;
+        const float2 back = both(-rstd * rstd * (dot / static_cast<float>(width)));
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
-            const int64_t column = threadIdx.x * kVec + c * step;
-            if (column < p.K) {
-                float n[kVec], u[kVec], w[kVec], res[kVec];
+            const int column = column0 + c * step;
+            if (column < width) {
+                Pairs n, u, w, r;
                 unpack8<kFp16>(x[c], n);
                 unpack8<kFp16>(g[c], u);
-                unpack8<kFp16>(r[c], res);
+                unpack8<kFp16>(res[c], r);
                 load_weight<kFp16, kWeightF32>(p.weight, column, w);
 #pragma unroll
-                for (int i = 0; i < kVec; ++i) {
-                    const float d = u[i] * w[i] - n[i] * rstd * mean;
-                    u[i] = p.grad_residual != nullptr ? fmaf(d, rstd, res[i]) : d * rstd;
-                }
-                *reinterpret_cast<uint4*>(p.grad_x + base + column) = pack8<kFp16>(u);
+                for (int i = 0; i < 4; ++i) r[i] = __ffma2_rn(n[i], back, __ffma2_rn(__fmul2_rn(u[i], w[i]), both(rstd), r[i]));
+                *reinterpret_cast<uint4*>(p.grad_x + base + column) = pack8<kFp16>(r);
             }
         }
     }
+    grid_launch_dependents();
+    if (blockDim.y > 1) {
+        // the CTA's rows first: one warp after the other adds its share in shared memory
+        for (int y = 0; y < static_cast<int>(blockDim.y); ++y) {
+            __syncthreads();
+            if (static_cast<int>(threadIdx.y) == y) {
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c) {
+                    const int column = column0 + c * step;
+                    if (column < width) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float2* const sum = reinterpret_cast<float2*>(total + column) + i;
+                            if (y > 0) dw[c][i] = __fadd2_rn(dw[c][i], *sum);
+                            *sum = dw[c][i];
+                        }
+                    }
+                }
+            }
+        }
+        if (threadIdx.y + 1 != blockDim.y) return;
+    }
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
-        const int64_t column = threadIdx.x * kVec + c * step;
-        if (column < p.K) {
+        const int column = column0 + c * step;
+        if (column < width) {
             float4* const to = reinterpret_cast<float4*>(p.partials + blockIdx.x * p.K + column);
-            to[0] = make_float4(dw[c][0], dw[c][1], dw[c][2], dw[c][3]);
-            to[1] = make_float4(dw[c][4], dw[c][5], dw[c][6], dw[c][7]);
+            to[0] = make_float4(dw[c][0].x, dw[c][0].y, dw[c][1].x, dw[c][1].y);
+            to[1] = make_float4(dw[c][2].x, dw[c][2].y, dw[c][3].x, dw[c][3].y);
         }
     }
 }
@@ -371,11 +470,12 @@ __global__ void __launch_bounds__(kMaxNormThreads) rms_norm_dgrad_kernel(const N
 constexpr int kSumWarps = 8;
 __global__ void __launch_bounds__(32 * kSumWarps) column_sum_kernel(const float* __restrict__ partials, float* __restrict__ out, int rows, int64_t K) {
     __shared__ float part[kSumWarps][33];
-    start_after_kernel_ahead();
+    grid_dependency_wait();   // launched behind the kernel that writes the partials, as its dependent
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t column = static_cast<int64_t>(blockIdx.x) * 32 + lane;
     float sum = 0.0f;
     if (column < K) {
+#pragma unroll 8
         for (int r = warp; r < rows; r += kSumWarps) sum += partials[r * K + column];
     }
     part[warp][lane] = sum;
@@ -388,10 +488,11 @@ __global__ void __launch_bounds__(32 * kSumWarps) column_sum_kernel(const float*
 
 // `overlap`: may start while the kernel ahead in the stream still runs
 template <class... Params, class... Args>
-bool launch_kernel(void (*kernel)(Params...), int64_t grid, int threads, cudaStream_t stream, bool overlap, Args... args) {
+bool launch_kernel(void (*kernel)(Params...), int64_t grid, dim3 block, size_t smem, cudaStream_t stream, bool overlap, Args... args) {
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(static_cast<unsigned>(grid));
-    config.blockDim = dim3(static_cast<unsigned>(threads));
+    config.blockDim = block;
+    config.dynamicSmemBytes = smem;
     config.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -403,19 +504,33 @@ bool launch_kernel(void (*kernel)(Params...), int64_t grid, int threads, cudaStr
 
 bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
-// Threads and chunks per thread for one row per CTA: as few chunks as 1024 threads allow when there are few rows (a row
-// is then a matter of latency), four per thread otherwise (independent loads, few threads at the barrier).
+// The threads of a row and the 8-channel chunks that each of them has. One warp up to 1024 channels; beyond, two chunks per
+// thread, one where there are few rows (a row is then a matter of latency), and four where 1024 threads need them. The numbers
+// come from the sizes alone, and with them the order of the sums.
 struct RowShape {
-    int threads, chunks;
+    int threads, rows, chunks;   // blockDim.x, blockDim.y
 };
 
-RowShape row_shape(int64_t M, int64_t K, int wanted) {
+constexpr int kSms = 148;   // of a B200
+
+RowShape row_shape(int64_t M, int64_t K) {
     const int64_t vectors = K / kVec;
-    int chunks = M <= 2 * device_info().sm_count ? 1 : wanted;
-    while (chunks > 1 && vectors < static_cast<int64_t>(chunks) * 32) chunks >>= 1;
+    const bool few = M <= 2 * kSms;
+    if (K <= kWarpRowWidth && !few) return {32, kRowsPerCta, vectors <= 32 ? 1 : vectors <= 64 ? 2 : 4};
+    int chunks = few ? 1 : 2;
     while ((vectors + chunks - 1) / chunks > kMaxNormThreads) chunks <<= 1;
     const int64_t threads = (vectors + chunks - 1) / chunks;
-    return {static_cast<int>((threads + 31) / 32 * 32), chunks};
+    return {static_cast<int>((threads + 31) / 32 * 32), 1, chunks};
+}
+
+// CTAs of the norm's backward pass: what an SM holds at 64 registers a thread (twice that with four chunks per warp), four at most, and two
+// rows each at least.
+int norm_grad_grid(int64_t M, const RowShape& shape) {
+    int64_t per_sm = 1024 / (shape.threads * shape.rows);
+    per_sm = per_sm > 4 ? 4 : per_sm < 1 ? 1 : per_sm;
+    if (shape.rows > 1 && shape.chunks == 4) per_sm = 2;
+    const int64_t wanted = (M + 2 * shape.rows - 1) / (2 * shape.rows);
+    return static_cast<int>(wanted < kSms * per_sm ? wanted : kSms * per_sm);
 }
 
 template <bool kFp16, bool kE5M2, bool kGate>
@@ -426,7 +541,7 @@ bool launch_tile(const void* x, void* q, float* scale, int64_t M, int64_t K, cud
     const int64_t grid = (tasks + kTileWarps - 1) / kTileWarps;
     if (column_warps > 0x7fffffff || grid > 0x7fffffff) return false;
     const auto kernel = rows == 4 ? tile_quantize_kernel<kFp16, kE5M2, kGate, 4> : tile_quantize_kernel<kFp16, kE5M2, kGate, 1>;
-    return launch_kernel(kernel, grid, 32 * kTileWarps, stream, overlap, static_cast<const uint16_t*>(x), static_cast<uint8_t*>(q), scale, M, K,
+    return launch_kernel(kernel, grid, dim3(32 * kTileWarps), 0, stream, overlap, static_cast<const uint16_t*>(x), static_cast<uint8_t*>(q), scale, M, K,
                          static_cast<int>(column_warps));
 }
 
@@ -441,28 +556,30 @@ bool dispatch_tile(const void* x, void* q, float* scale, int64_t M, int64_t K, b
 
 template <bool kFp16, bool kWeightF32, bool kE5M2>
 bool launch_norm(const NormParams& p, cudaStream_t stream) {
-    const RowShape shape = row_shape(p.M, p.K, 4);
-    const auto kernel = shape.chunks == 1   ? rms_norm_fp8_kernel<kFp16, kWeightF32, kE5M2, 1>
-                        : shape.chunks == 2 ? rms_norm_fp8_kernel<kFp16, kWeightF32, kE5M2, 2>
-                                            : rms_norm_fp8_kernel<kFp16, kWeightF32, kE5M2, 4>;
-    return launch_kernel(kernel, p.M, shape.threads, stream, true, p);
+    const RowShape shape = row_shape(p.M, p.K);
+    // Two rows at once where there are rows enough to fill the SMs all the same: 8192 x 4096 with a residual 41.4 against 38.4 us,
+    // without 26.1 against 25.1; 500 x 5120 5.1 against 5.7.
+    const bool two = p.M >= 2048 && shape.rows == 1 && shape.chunks <= 2;
+    const auto kernel = shape.chunks == 1   ? (two ? rms_norm_fp8_kernel<kFp16, kWeightF32, kE5M2, 1, 2> : rms_norm_fp8_kernel<kFp16, kWeightF32, kE5M2, 1, 1>)
+                        : shape.chunks == 2 ? (two ? rms_norm_fp8_kernel<kFp16, kWeightF32, kE5M2, 2, 2> : rms_norm_fp8_kernel<kFp16, kWeightF32, kE5M2, 2, 1>)
+                                            : rms_norm_fp8_kernel<kFp16, kWeightF32, kE5M2, 4, 1>;
+    const int64_t rows = shape.rows * (two ? 2 : 1);
+    return launch_kernel(kernel, (p.M + rows - 1) / rows, dim3(shape.threads, shape.rows), 0, stream, true, p);
 }
 
 template <bool kFp16, bool kWeightF32>
-bool launch_norm_grad(const NormGradParams& p, int grid, cudaStream_t stream) {
-    const RowShape shape = row_shape(p.M, p.K, 2);
-    const auto kernel = shape.chunks == 1   ? rms_norm_dgrad_kernel<kFp16, kWeightF32, 1>
-                        : shape.chunks == 2 ? rms_norm_dgrad_kernel<kFp16, kWeightF32, 2>
-                                            : rms_norm_dgrad_kernel<kFp16, kWeightF32, 4>;
-    return launch_kernel(kernel, grid, shape.threads, stream, true, p);
-}
-
-// CTAs of the norm's backward pass: at most two per SM of a B200 (their registers hold two), at least four rows each. A
-// constant and not the device's count, so that the size of the scratch and the order of the sums do not depend on the device.
-constexpr int64_t kNormGradCtas = 296;
-int norm_grad_grid(int64_t M) {
-    const int64_t wanted = (M + 3) / 4;
-    return static_cast<int>(wanted < kNormGradCtas ? wanted : kNormGradCtas);
+bool launch_norm_grad(const NormGradParams& p, float* grad_weight, cudaStream_t stream) {
+    const RowShape shape = row_shape(p.M, p.K);
+    const int grid = norm_grad_grid(p.M, shape);
+    const auto kernel = shape.chunks == 1   ? rms_norm_dgrad_kernel<kFp16, kWeightF32, 1, kMaxNormThreads>
+                        : shape.chunks == 2 ? rms_norm_dgrad_kernel<kFp16, kWeightF32, 2, kMaxNormThreads>
+                        : shape.rows > 1    ? rms_norm_dgrad_kernel<kFp16, kWeightF32, 4, 32 * kRowsPerCta>
+                                            : rms_norm_dgrad_kernel<kFp16, kWeightF32, 4, kMaxNormThreads>;
+    const size_t smem = shape.rows > 1 ? static_cast<size_t>(p.K) * 4 : 0;
+    // An ordinary launch: a persistent grid that starts among the CTAs of the kernel ahead is spread unevenly over the SMs (84 against 68 us
+    // at 8192 x 4096).
+    if (!launch_kernel(kernel, grid, dim3(shape.threads, shape.rows), smem, stream, false, p)) return false;
+    return launch_kernel(column_sum_kernel, (p.K + 31) / 32, dim3(32 * kSumWarps), 0, stream, true, static_cast<const float*>(p.partials), grad_weight, grid, p.K);
 }
 
 }  // namespace
@@ -496,7 +613,7 @@ extern "C" bool launch_silu_mul_dgrad(const void* grad, const void* gate_up, voi
     const int64_t grid = (chunks + 255) / 256;
     if (grid > 0x7fffffff) return false;
     const auto kernel = input_fp16 != 0 ? silu_mul_dgrad_kernel<true> : silu_mul_dgrad_kernel<false>;
-    return launch_kernel(kernel, grid, 256, stream, true, static_cast<const uint16_t*>(grad), static_cast<const uint16_t*>(gate_up),
+    return launch_kernel(kernel, grid, dim3(256), 0, stream, true, static_cast<const uint16_t*>(grad), static_cast<const uint16_t*>(gate_up),
                          static_cast<uint16_t*>(grad_gate_up), chunks, row_chunks);
 }
 
@@ -522,7 +639,8 @@ extern "C" bool launch_rms_norm_fp8(const void* x, const void* residual, const v
 }
 
 extern "C" int64_t feather_rms_norm_dgrad_partial_floats(int64_t M, int64_t K) {
-    return M <= 0 || K <= 0 ? 0 : norm_grad_grid(M) * K;
+    if (M <= 0 || K <= 0 || K > kMaxNormWidth) return 0;
+    return norm_grad_grid(M, row_shape(M, K)) * K;
 }
 
 extern "C" bool launch_rms_norm_dgrad(const void* grad, const void* x, const void* weight, const float* rstd, const void* grad_residual, void* grad_x,
@@ -533,13 +651,8 @@ extern "C" bool launch_rms_norm_dgrad(const void* grad, const void* x, const voi
     const NormGradParams p{static_cast<const uint16_t*>(grad), static_cast<const uint16_t*>(x), weight, rstd, static_cast<const uint16_t*>(grad_residual),
                            static_cast<uint16_t*>(grad_x), partials, M, K};
     
-    const int grid = norm_grad_grid(M);
-    bool ok;
     if (input_fp16 != 0) {
-        ok = weight_f32 != 0 ? launch_norm_grad<true, true>(p, grid, stream) : launch_norm_grad<true, false>(p, grid, stream);
-    } else {
-        ok = weight_f32 != 0 ? launch_norm_grad<false, true>(p, grid, stream) : launch_norm_grad<false, false>(p, grid, stream);
+        return weight_f32 != 0 ? launch_norm_grad<true, true>(p, grad_weight, stream) : launch_norm_grad<true, false>(p, grad_weight, stream);
     }
-    if (!ok) return false;
-    return launch_kernel(column_sum_kernel, (K + 31) / 32, 32 * kSumWarps, stream, true, static_cast<const float*>(partials), grad_weight, grid, K);
+    return weight_f32 != 0 ? launch_norm_grad<false, true>(p, grad_weight, stream) : launch_norm_grad<false, false>(p, grad_weight, stream);
 }

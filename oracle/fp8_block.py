@@ -36,15 +36,15 @@ def quantize(y: torch.Tensor, dtype: torch.dtype) -> tuple[torch.Tensor, torch.T
 
 
 def quantize_f32(x: torch.Tensor, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
-    """The quantizer's own float32 steps: one inverse per block, one product per element, one rounding."""
+    """The quantizer's own float32 steps: a reciprocal and two products per block, one product per element, one rounding."""
     m, k = x.shape
     kb = -(-k // BLOCK)
     padded = torch.zeros(m, kb * BLOCK)
     padded[:, :k] = x.float()
     top = padded.view(m, kb, BLOCK).abs().amax(2).clamp(min=1e-30 * TOP[dtype])
-    inverse = torch.tensor(TOP[dtype]) / top
+    inverse = top.reciprocal() * TOP[dtype]
     q = (padded.view(m, kb, BLOCK) * inverse[:, :, None]).view(m, kb * BLOCK)[:, :k].to(dtype)
-    return q, (top / TOP[dtype]).t().contiguous()
+    return q, (top * torch.tensor(1 / TOP[dtype])).t().contiguous()
 
 
 def weight_values(w: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:

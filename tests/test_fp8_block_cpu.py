@@ -82,9 +82,9 @@ def test_launchers_refuse_bad_arguments_without_a_device(lib):
 
 
 def test_scratch_of_the_norms_weight_gradient(lib):
-    # four rows per CTA at least, 296 CTAs at most
-    for m, ctas in ((0, 0), (1, 1), (4, 1), (5, 2), (1184, 296), (1185, 296), (100000, 296)):
-        assert lib.feather_rms_norm_dgrad_partial_floats(m, 272) == ctas * 272
+    # a row of partials per CTA: two rows of the input each at least, and at most four CTAs per SM
+    for m, k, ctas in ((0, 272, 0), (1, 272, 1), (3, 272, 2), (200, 4096, 100), (100000, 2048, 592), (100000, 4096, 592), (100000, 32768, 148), (100000, 8192, 296), (100000, 512, 592)):
+        assert lib.feather_rms_norm_dgrad_partial_floats(m, k) == ctas * k
 
 
 def test_norm_gradient_formula_against_differences():
