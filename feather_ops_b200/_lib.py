@@ -57,8 +57,9 @@ PROTOTYPES = {
     "launch_fp8_block_mm": (_c_bool, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _c_bool, _c_int, _c_int, _c_int, _ptr]),
     "launch_fp8_block_linear": (
         _c_bool,
-        [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _c_bool, _c_int, _c_int, _c_int, _c_int, _ptr],
+        [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _c_bool, _c_int, _c_int, _c_int, _c_int, _ptr],
     ),
+    "feather_fp8_block_linear_scratch_bytes": (_i64, [_i64, _i64]),
     "feather_fp8_block_mm_status": (_c_int, [_ptr]),
     "launch_rms_norm_fp8": (_c_bool, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, ctypes.c_float, _c_int, _c_int, _c_int, _ptr]),
     "launch_rms_norm_dgrad": (_c_bool, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _c_int, _c_int, _ptr]),

@@ -13,13 +13,12 @@
 //     so that a few tokens cost no padding to 128 rows. K is split over the CTAs of a cluster, which add their partial sums through
 //     distributed shared memory in a fixed order.
 //   * pair_kernel: 256 tokens x 256 outputs per CTA pair, persistent.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
 
 #include "feather_host.h"
+#include "fp8_block.cuh"
 #include "sm100_ptx.cuh"
 
 namespace feather {
@@ -29,13 +28,18 @@ bool launch_fp8_block_quantize_ahead(const void* x, void* q, float* scale, int64
 
 namespace f8mm {
 
-constexpr int kBlock = 128;          // depth of a k block = channels per scale
+using f8::kBlock;                    // depth of a k block = channels per scale
 constexpr int kTileBytes = 128 * 128;
+constexpr int kQuantizeRows = 8;     // up to so many tokens the product quantizes its activation itself ...
+constexpr int kQuantizeWarps = 8;    // ... with so many warps, a k block each in turn
 constexpr int kMaxSplits = 8;        // CTAs of a cluster along the contraction (the largest portable cluster)
 
 __device__ uint32_t g_status[2];
 
 struct Params {
+    const uint16_t* x;       // small kernel that quantizes: the 16-bit activation
+    int depth;
+    bool x_fp16, x_e5m2;
     const float* a_scale;
     const float* w_scale;
     const uint16_t* bias;
@@ -146,14 +150,43 @@ __device__ __forceinline__ void fma2(float2& d, uint32_t v0, uint32_t v1, float 
         : "r"(v0), "r"(v1), "f"(s0), "f"(s1));
 }
 
+// Codes of one k block of the activation into the swizzled rows of an operand tile, and sa * sw of its tokens. Two tokens per pass, 16
+// lanes each; no branch between the passes, so that their chains of shuffles overlap.
+constexpr int kQuantizePasses = kQuantizeRows / 2;
+
+template <bool kFp16, bool kE5M2>
+__device__ __forceinline__ void quantize_passes(const uint4 (&in)[kQuantizePasses], int live, float sw, uint8_t* rows, float* product) {
+    const int lane = static_cast<int>(threadIdx.x) % 32;
+    const int chunk = lane % 16;
+    uint2 codes[kQuantizePasses];
+    float scale[kQuantizePasses];
+#pragma unroll
+    for (int t = 0; t < kQuantizePasses; ++t) {
+        f8::Pairs v;
+        f8::unpack8<kFp16>(in[t], v);
+        codes[t] = f8::encode_block<kE5M2>(v, f8::max_magnitude_packed<kFp16>(in[t]), scale[t]);
+    }
+#pragma unroll
+    for (int t = 0; t < kQuantizePasses; ++t) {
+        const int token = 2 * t + lane / 16;
+        if (token < live) {
+            *reinterpret_cast<uint2*>(rows + sw128_offset(token, chunk / 2) + chunk % 2 * 8) = codes[t];
+            if (chunk == 0) product[token] = scale[t] * sw;
+        }
+    }
+}
+
 // ---------------------------------------------------------------------------------------------------------
 // A few tokens: D[128 outputs, T tokens]
 // ---------------------------------------------------------------------------------------------------------
-// T tokens per tile. Up to 32 tokens the weight is the UMMA's M side: lanes of tensor memory are outputs, columns tokens,
+// T tokens per tile. With kQuantize (at most 8 tokens) the activation comes in 16 bits and eight warps write its codes into the operand
+// ring themselves, a k block each in turn: every CTA quantizes the tokens again, which costs no time beside the weight, and a launch is
+// saved, 3.4 us of the host's 11. With more tokens it does not keep up (24 x 5120 x 5120 17.3 us, 12.4 with a quantizer in front).
+// Up to 32 tokens the weight is the UMMA's M side: lanes of tensor memory are outputs, columns tokens,
 // and a column's scale comes from shared memory. With T = 128 the tokens are the M side, so that a lane has one scale per
 // k block and the registers of a warp are outputs. (64 tokens as columns were never faster than 128 lanes: 64 x 5120 x 5120
 // in three K splits 13.0 us against 10.9.)
-template <int T>
+template <int T, bool kQuantize>
 struct SmallShape {
     static constexpr bool kTokenLanes = T == 128;
     static constexpr int kWidth = kTokenLanes ? 128 : T;                 // columns of an accumulator
@@ -161,7 +194,8 @@ struct SmallShape {
     static constexpr int kGroups = kWidth / kColumns;
     static constexpr int kTeams = kTokenLanes ? 1 : 2;                   // teams take the k blocks in turn
     static constexpr int kWarps = 4 * kGroups * kTeams;
-    static constexpr int kThreads = 32 * (kWarps + 3);                   // the last three load, multiply and bring the scales
+    static constexpr int kScaleWarps = kQuantize ? kQuantizeWarps : 1;
+    static constexpr int kThreads = 32 * (kWarps + 2 + kScaleWarps);     // the last ones load, multiply, and bring the scales or quantize
     static constexpr int kStageBytes = kTileBytes + T * 128;
     static constexpr int kStages = T == 16 ? 11 : T == 32 ? 10 : 6;
     static constexpr int kSlots = T == 128 ? 4 : 8;                      // accumulators in tensor memory
@@ -178,13 +212,14 @@ struct SmallShape {
     static constexpr int kDynamic = kTotal + 1024;
     static_assert(kTeams * T * kPitch * 4 <= kStages * kStageBytes, "the partial sums are laid out in the operand ring");
     static_assert(kDynamic <= 227 * 1024 && kTmemColumns <= 512, "what an SM holds");
+    static_assert(!kQuantize || T == 16, "the warps that quantize have registers for 8 tokens");
     static_assert(kSlots % kTeams == 0, "a team's accumulators are its own");
 };
 
-template <int T, bool kBackward, bool kOutBf16>
-__global__ void __launch_bounds__(SmallShape<T>::kThreads, 1)
+template <int T, bool kBackward, bool kOutBf16, bool kQuantize>
+__global__ void __launch_bounds__((SmallShape<T, kQuantize>::kThreads), 1)
 small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const Params p) {
-    using L = SmallShape<T>;
+    using L = SmallShape<T, kQuantize>;
     extern __shared__ uint8_t smem_dyn[];
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~static_cast<uintptr_t>(1023));
     uint64_t* const full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
@@ -200,7 +235,7 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
     if (threadIdx.x == 0) {
         *abort_flag = 0u;
         for (int s = 0; s < L::kStages; ++s) {
-            mbar_init(&full[s], 1);
+            mbar_init(&full[s], kQuantize ? 2 : 1);
             mbar_init(&empty[s], 1);
         }
         for (int s = 0; s < L::kSlots; ++s) {
@@ -211,7 +246,7 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
     }
     if (warp == L::kWarps) {
         if (elect_one()) {
-            tma_prefetch_desc(&map_a);
+            if constexpr (!kQuantize) tma_prefetch_desc(&map_a);
             tma_prefetch_desc(&map_w);
         }
         __syncwarp();
@@ -239,7 +274,7 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
         if (elect_one()) {
             const auto load_weight = [&](int i, int slot) {
                 const int depth0 = (kb_begin + i) * kBlock;
-                mbar_arrive_expect_tx(&full[slot], L::kStageBytes);
+                mbar_arrive_expect_tx(&full[slot], kQuantize ? kTileBytes : L::kStageBytes);
                 tma_load_2d(smem + slot * L::kStageBytes, &map_w, &full[slot], kBackward ? n0 : depth0, kBackward ? depth0 : n0);
             };
             // behind the quantizer the weight fills the ring while that runs
@@ -250,7 +285,7 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
             for (int i = 0; i < blocks; ++i) {
                 if (!guard.wait(&empty[slot.idx], slot.phase ^ 1u, kSiteLoadEmpty)) break;
                 if (i >= early) load_weight(i, static_cast<int>(slot.idx));
-                tma_load_2d(smem + slot.idx * L::kStageBytes + kTileBytes, &map_a, &full[slot.idx], (kb_begin + i) * kBlock, m0);
+                if constexpr (!kQuantize) tma_load_2d(smem + slot.idx * L::kStageBytes + kTileBytes, &map_a, &full[slot.idx], (kb_begin + i) * kBlock, m0);
                 slot.advance(L::kStages);
             }
         }
@@ -275,6 +310,54 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
                 slot.advance(L::kStages);
                 out.advance(L::kSlots);
             }
+        }
+    } else if (kQuantize && warp >= L::kWarps + 2) {
+        // ---------------------------------------------------------------------- codes and scales, a k block per warp in turn
+        const int first = warp - (L::kWarps + 2);
+        float* const products = reinterpret_cast<float*>(smem + L::kScaleOff);
+        const float* const w_scale = p.w_scale + tile_n * p.w_scale_out + kb_begin * p.w_scale_block;
+        const int chunk = lane % 16;                          // 8 channels of the block
+        const uint16_t* const x = p.x + static_cast<int64_t>(m0) * p.depth + chunk * 8;
+        uint4 in[kQuantizePasses];
+        float sw = 0.0f;
+        const auto fetch = [&](int i) {
+            if (i >= blocks) return;
+            const int column = (kb_begin + i) * kBlock;
+            sw = __ldg(w_scale + i * p.w_scale_block);
+#pragma unroll
+            for (int t = 0; t < kQuantizePasses; ++t) {
+                const int token = 2 * t + lane / 16;
+                in[t] = token < live && column + chunk * 8 < p.depth ? f8::load16(x + static_cast<int64_t>(token) * p.depth + column) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        // the ring's rows past the last token are zero, once and for all
+        const int spare = (T - live) * 8;
+        for (int i = first * 32 + lane; i < spare * L::kStages; i += 32 * L::kScaleWarps) {
+            *reinterpret_cast<uint4*>(smem + i / spare * L::kStageBytes + kTileBytes + live * 128 + i % spare * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * L::kScaleWarps) : "memory");
+        grid_dependency_wait();
+        fetch(first);
+        for (int i = first; i < blocks; i += L::kScaleWarps) {
+            const int slot = i % L::kStages, at = i % L::kSlots, before = i - L::kSlots;
+            if (!warp_wait(guard, &empty[slot], (static_cast<uint32_t>(i / L::kStages) & 1u) ^ 1u, kSiteOperandEmpty)) break;
+            // the accumulator's previous product is complete, as for the scale warp below
+            if (before >= 0 && !warp_wait(guard, &tmem_full[before % L::kSlots], static_cast<uint32_t>(before / L::kSlots) & 1u, kSiteTmemFull)) break;
+            uint8_t* const rows = smem + slot * L::kStageBytes + kTileBytes;
+            float* const product = products + i % (2 * L::kSlots) * T;
+            if (p.x_fp16) {
+                p.x_e5m2 ? quantize_passes<true, true>(in, live, sw, rows, product) : quantize_passes<true, false>(in, live, sw, rows, product);
+            } else {
+                p.x_e5m2 ? quantize_passes<false, true>(in, live, sw, rows, product) : quantize_passes<false, false>(in, live, sw, rows, product);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&full[slot]);
+                mbar_arrive(&tmem_full[at]);
+            }
+            fetch(i + L::kScaleWarps);
         }
     } else if (warp == L::kWarps + 2) {
         // ---------------------------------------------------------------------- scales, kBatch k blocks at a time
@@ -397,7 +480,7 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
 #pragma unroll
             for (int j = 0; j < 4; ++j) bias[j] = bits_to_float<kOutBf16>(__ldg(p.bias + column + j));
         }
-        for (int t = rank * share + warp; t < token_end; t += L::kWarps + 3) {
+        for (int t = rank * share + warp; t < token_end; t += L::kThreads / 32) {
             float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             for (int s = 0; s < splits; ++s) {
                 const uint32_t part = map_to_cta(smem_u32(smem), static_cast<uint32_t>(s)) + (t * L::kPitch + 4 * lane) * 4;
@@ -751,6 +834,8 @@ struct Args {
     int64_t M, N, K;   // N and K: the weight's axes
     bool transposed_b, a_e5m2, w_e5m2, out_bf16;
     bool weight_ready;   // the kernel ahead in the stream is this library's quantizer, launched in the same call after all else had finished
+    const uint16_t* x;   // not null: the small kernel quantizes it (a and a_scale are unused)
+    bool x_fp16;
     cudaStream_t stream;
 
     int64_t width() const { return transposed_b ? K : N; }
@@ -759,6 +844,10 @@ struct Args {
 
 Params make_params(const Args& args) {
     Params p{};
+    p.x = args.x;
+    p.depth = static_cast<int>(args.depth());
+    p.x_fp16 = args.x_fp16;
+    p.x_e5m2 = args.a_e5m2;
     const int64_t scale_pitch = (args.K + kBlock - 1) / kBlock;
     p.a_scale = args.a_scale;
     p.w_scale = args.w_scale;
@@ -772,22 +861,25 @@ Params make_params(const Args& args) {
     return p;
 }
 
-bool make_maps(const Args& args, int a_rows, int w_rows, CUtensorMap& map_a, CUtensorMap& map_w) {
-    const uint64_t a_dims[2] = {static_cast<uint64_t>(args.depth()), static_cast<uint64_t>(args.M)};
-    const uint64_t a_strides[1] = {static_cast<uint64_t>(args.depth())};
-    const uint32_t a_box[2] = {kBlock, static_cast<uint32_t>(a_rows)};
-    const uint64_t w_dims[2] = {static_cast<uint64_t>(args.K), static_cast<uint64_t>(args.N)};
-    const uint64_t w_strides[1] = {static_cast<uint64_t>(args.K)};
-    const uint32_t w_box[2] = {128, static_cast<uint32_t>(w_rows)};
-    return encode_map(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, args.a, a_dims, a_strides, a_box, CU_TENSOR_MAP_SWIZZLE_128B) &&
-           encode_map(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, args.w, w_dims, w_strides, w_box, CU_TENSOR_MAP_SWIZZLE_128B);
+bool make_map_a(const Args& args, int rows, CUtensorMap& map) {
+    const uint64_t dims[2] = {static_cast<uint64_t>(args.depth()), static_cast<uint64_t>(args.M)};
+    const uint64_t strides[1] = {static_cast<uint64_t>(args.depth())};
+    const uint32_t box[2] = {kBlock, static_cast<uint32_t>(rows)};
+    return encode_map(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, args.a, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+bool make_map_w(const Args& args, int rows, CUtensorMap& map) {
+    const uint64_t dims[2] = {static_cast<uint64_t>(args.K), static_cast<uint64_t>(args.N)};
+    const uint64_t strides[1] = {static_cast<uint64_t>(args.K)};
+    const uint32_t box[2] = {128, static_cast<uint32_t>(rows)};
+    return encode_map(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, args.w, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 uint32_t format(bool e5m2) { return e5m2 ? kFmtE5M2 : kFmtE4M3; }
 
-template <int T, bool kBackward, bool kOutBf16>
+template <int T, bool kQuantize>
 cudaLaunchConfig_t small_config(cudaLaunchAttribute* attr, int64_t grid, int splits) {
-    using L = SmallShape<T>;
+    using L = SmallShape<T, kQuantize>;
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(static_cast<unsigned>(grid));
     config.blockDim = dim3(L::kThreads);
@@ -803,14 +895,14 @@ cudaLaunchConfig_t small_config(cudaLaunchAttribute* attr, int64_t grid, int spl
 
 // How many clusters of `splits` CTAs the device holds at once (0: none, or the kernel cannot be prepared). Asked once per
 // device: clusters live within a GPC, so 148 SMs hold 45 clusters of three and 15 of eight.
-template <int T, bool kBackward, bool kOutBf16>
+template <int T, bool kBackward, bool kOutBf16, bool kQuantize>
 int small_clusters(int splits) {
     static PerDeviceState resident[kMaxSplits + 1];
     return resident[splits].get([&] {
-        auto* const kernel = &small_kernel<T, kBackward, kOutBf16>;
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SmallShape<T>::kDynamic) != cudaSuccess) return 0;
+        auto* const kernel = &small_kernel<T, kBackward, kOutBf16, kQuantize>;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SmallShape<T, kQuantize>::kDynamic) != cudaSuccess) return 0;
         cudaLaunchAttribute attr[2];
-        const cudaLaunchConfig_t config = small_config<T, kBackward, kOutBf16>(attr, device_info().sm_count / splits * splits, splits);
+        const cudaLaunchConfig_t config = small_config<T, kQuantize>(attr, device_info().sm_count / splits * splits, splits);
         int clusters = 0;
         if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &config) != cudaSuccess) {
             (void)cudaGetLastError();
@@ -820,11 +912,16 @@ int small_clusters(int splits) {
     });
 }
 
-template <int T, bool kBackward, bool kOutBf16>
+template <int T, bool kBackward, bool kOutBf16, bool kQuantize>
 bool launch_small(const Args& args, int splits) {
-    if (small_clusters<T, kBackward, kOutBf16>(splits) <= 0) return false;
+    if (small_clusters<T, kBackward, kOutBf16, kQuantize>(splits) <= 0) return false;
     CUtensorMap map_a, map_w;
-    if (!make_maps(args, T, 128, map_a, map_w)) return false;
+    if (!make_map_w(args, 128, map_w)) return false;
+    if constexpr (kQuantize) {
+        map_a = map_w;   // unused
+    } else {
+        if (!make_map_a(args, T, map_a)) return false;
+    }
     Params p = make_params(args);
     const int64_t tiles_m = (args.M + T - 1) / T, tiles_n = (args.width() + 127) / 128;
     if (tiles_m * tiles_n * splits > 0x7fffffff) return false;
@@ -832,15 +929,15 @@ bool launch_small(const Args& args, int splits) {
     p.tiles_n = static_cast<int>(tiles_n);
     p.splits = splits;
     p.weight_ready = args.weight_ready;
-    p.idesc = SmallShape<T>::kTokenLanes ? make_idesc(kAccF32, format(args.a_e5m2), format(args.w_e5m2), 128, 128) | (kBackward ? kIdescBMajorMN : 0u)
+    p.idesc = SmallShape<T, kQuantize>::kTokenLanes ? make_idesc(kAccF32, format(args.a_e5m2), format(args.w_e5m2), 128, 128) | (kBackward ? kIdescBMajorMN : 0u)
                                          : make_idesc(kAccF32, format(args.w_e5m2), format(args.a_e5m2), 128, T) | (kBackward ? kIdescAMajorMN : 0u);
     cudaLaunchAttribute attr[2];
-    cudaLaunchConfig_t config = small_config<T, kBackward, kOutBf16>(attr, tiles_m * tiles_n * splits, splits);
+    cudaLaunchConfig_t config = small_config<T, kQuantize>(attr, tiles_m * tiles_n * splits, splits);
     config.stream = args.stream;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     config.numAttrs = 2;
-    return cudaLaunchKernelEx(&config, &small_kernel<T, kBackward, kOutBf16>, map_a, map_w, p) == cudaSuccess;
+    return cudaLaunchKernelEx(&config, &small_kernel<T, kBackward, kOutBf16, kQuantize>, map_a, map_w, p) == cudaSuccess;
 }
 
 template <bool kBackward, bool kOutBf16>
@@ -870,7 +967,7 @@ bool launch_pair(const Args& args) {
     });
     if (pairs <= 0) return false;
     CUtensorMap map_a, map_w, map_c;
-    if (!make_maps(args, 128, kBackward ? 128 : kPairN / 2, map_a, map_w)) return false;
+    if (!make_map_a(args, 128, map_a) || !make_map_w(args, kBackward ? 128 : kPairN / 2, map_w)) return false;
     const uint64_t c_dims[2] = {static_cast<uint64_t>(args.width()), static_cast<uint64_t>(args.M)};
     const uint64_t c_strides[1] = {static_cast<uint64_t>(args.width()) * 2};
     const uint32_t c_box[2] = {32, 32};
@@ -901,29 +998,31 @@ bool launch_pair(const Args& args) {
 // Microseconds that a product takes on the small kernel with T tokens per tile and `splits` K splits, or a negative number
 // where the clusters would not be resident at once. Per launch 3.5; per k block of a CTA 0.29 with 16 or 32 tokens and 0.45 with
 // 128 (every SM busy; the activation tile then is as large as the weight's); the exchange of the partial sums 1.0 and 1.8.
-template <int T, bool kBackward, bool kOutBf16>
+template <int T, bool kBackward, bool kOutBf16, bool kQuantize>
 double small_cost(const Args& args, int splits) {
     const int64_t num_kb = (args.depth() + kBlock - 1) / kBlock;
     const int64_t tiles = (args.M + T - 1) / T * ((args.width() + 127) / 128);
-    const int clusters = splits > num_kb ? 0 : small_clusters<T, kBackward, kOutBf16>(splits);
+    const int clusters = splits > num_kb ? 0 : small_clusters<T, kBackward, kOutBf16, kQuantize>(splits);
     if (clusters <= 0 || (splits > 1 && tiles > clusters)) return -1.0;
     const double rounds = static_cast<double>((tiles + clusters - 1) / clusters);
     return 3.5 + rounds * static_cast<double>((num_kb + splits - 1) / splits) * (T == 128 ? 0.45 : 0.29) + (splits == 1 ? 0.0 : T == 128 ? 1.8 : 1.0);
 }
 
-template <int T, bool kBackward, bool kOutBf16>
+template <int T, bool kBackward, bool kOutBf16, bool kQuantize>
 bool launch_best_small(const Args& args, double pair_cost) {
     int best = 1;
-    double best_cost = small_cost<T, kBackward, kOutBf16>(args, 1);
+    double best_cost = small_cost<T, kBackward, kOutBf16, kQuantize>(args, 1);
     for (int splits = 2; splits <= kMaxSplits; ++splits) {
-        const double cost = small_cost<T, kBackward, kOutBf16>(args, splits);
+        const double cost = small_cost<T, kBackward, kOutBf16, kQuantize>(args, splits);
         if (cost >= 0.0 && cost < best_cost) {
             best = splits;
             best_cost = cost;
         }
     }
-    if (best_cost > pair_cost) return launch_pair<kBackward, kOutBf16>(args);
-    return launch_small<T, kBackward, kOutBf16>(args, best);
+    if constexpr (T == 128) {
+        if (best_cost > pair_cost) return launch_pair<kBackward, kOutBf16>(args);
+    }
+    return launch_small<T, kBackward, kOutBf16, kQuantize>(args, best);
 }
 
 // Up to 16 and 32 tokens their own tiles, above that 128 tokens per tile or the pair kernel, whichever the model says: a round of the
@@ -932,13 +1031,16 @@ bool launch_best_small(const Args& args, double pair_cost) {
 template <bool kBackward, bool kOutBf16>
 bool launch(const Args& args) {
     constexpr double kNever = 1e30;
-    if (args.M <= 16) return launch_best_small<16, kBackward, kOutBf16>(args, kNever);
-    if (args.M <= 32) return launch_best_small<32, kBackward, kOutBf16>(args, kNever);
+    if (args.x != nullptr) {
+        return launch_best_small<16, kBackward, kOutBf16, true>(args, kNever);
+    }
+    if (args.M <= 16) return launch_best_small<16, kBackward, kOutBf16, false>(args, kNever);
+    if (args.M <= 32) return launch_best_small<32, kBackward, kOutBf16, false>(args, kNever);
     const int pairs = device_info().sm_count / 2;
     const int64_t tiles = (args.M + 255) / 256 * ((args.width() + kPairN - 1) / kPairN);
     const int64_t num_kb = (args.depth() + kBlock - 1) / kBlock;
     const double pair_cost = 4.0 + static_cast<double>((tiles + pairs - 1) / pairs) * (0.57 * static_cast<double>(num_kb) + 1.0);
-    return launch_best_small<128, kBackward, kOutBf16>(args, pair_cost);
+    return launch_best_small<128, kBackward, kOutBf16, false>(args, pair_cost);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -948,8 +1050,9 @@ bool valid(const Args& args) {
     if (args.M < 0 || args.N <= 0 || args.K <= 0 || args.M > kMost || args.N > kMost || args.K > kMost || args.N % 16 != 0 || args.K % 16 != 0) return false;
     if (args.transposed_b && args.bias != nullptr) return false;
     if (args.M == 0) return true;
-    if (args.a == nullptr || args.a_scale == nullptr || args.w == nullptr || args.w_scale == nullptr || args.c == nullptr) return false;
-    return aligned16(args.a) && aligned16(args.w) && aligned16(args.c);
+    const bool codes = args.a != nullptr && args.a_scale != nullptr && aligned16(args.a);
+    if (!(args.x != nullptr ? aligned16(args.x) : codes) || args.w == nullptr || args.w_scale == nullptr || args.c == nullptr) return false;
+    return aligned16(args.w) && aligned16(args.c);
 }
 
 bool launch(const Args& args) {
@@ -965,16 +1068,30 @@ extern "C" bool launch_fp8_block_mm(const uint8_t* a, const float* a_scale, cons
                                     int64_t M, int64_t N, int64_t K, bool transposed_b, int a_e5m2, int w_e5m2, int output_dtype, cudaStream_t stream) {
     using namespace feather::f8mm;
     if (output_dtype != 0 && output_dtype != 1) return false;
-    const Args args{a, a_scale, w, w_scale, bias, c, M, N, K, transposed_b, a_e5m2 != 0, w_e5m2 != 0, output_dtype == 1, false, stream};
+    const Args args{a, a_scale, w, w_scale, bias, c, M, N, K, transposed_b, a_e5m2 != 0, w_e5m2 != 0, output_dtype == 1, false, nullptr, false, stream};
     return valid(args) && launch(args);
 }
 
-extern "C" bool launch_fp8_block_linear(const void* x, uint8_t* q, float* q_scale, const uint8_t* w, const float* w_scale, const uint16_t* bias, uint16_t* c,
-                                        int64_t M, int64_t N, int64_t K, bool transposed_b, int input_fp16, int q_e5m2, int w_e5m2, int output_dtype,
+extern "C" int64_t feather_fp8_block_linear_scratch_bytes(int64_t M, int64_t depth) {
+    using namespace feather::f8mm;
+    return M <= kQuantizeRows || depth <= 0 ? 0 : M * (depth + 4 * ((depth + kBlock - 1) / kBlock));
+}
+
+extern "C" bool launch_fp8_block_linear(const void* x, void* scratch, const uint8_t* w, const float* w_scale, const uint16_t* bias, uint16_t* c, int64_t M,
+                                        int64_t N, int64_t K, bool transposed_b, int input_fp16, int q_e5m2, int w_e5m2, int output_dtype,
                                         cudaStream_t stream) {
     using namespace feather::f8mm;
     if (output_dtype != 0 && output_dtype != 1) return false;
-    const Args args{q, q_scale, w, w_scale, bias, c, M, N, K, transposed_b, q_e5m2 != 0, w_e5m2 != 0, output_dtype == 1, true, stream};
+    Args args{nullptr, nullptr, w, w_scale, bias, c, M, N, K, transposed_b, q_e5m2 != 0, w_e5m2 != 0, output_dtype == 1, false, nullptr, input_fp16 != 0, stream};
+    if (M <= kQuantizeRows) {
+        args.x = static_cast<const uint16_t*>(x);
+        return valid(args) && launch(args);
+    }
+    uint8_t* const q = static_cast<uint8_t*>(scratch);
+    float* const q_scale = reinterpret_cast<float*>(q + M * args.depth());   // a row is a multiple of 16 bytes
+    args.a = q;
+    args.a_scale = q_scale;
+    args.weight_ready = true;
     return valid(args) && feather::launch_fp8_block_quantize_ahead(x, q, q_scale, M, args.depth(), input_fp16, q_e5m2, stream) && launch(args);
 }
 

@@ -423,7 +423,7 @@ Tensor fp8_block_mm(const Tensor& a, const Tensor& a_scale, const Tensor& weight
     return c;
 }
 
-// Quantizer and product in one call; the codes and their scales are scratch.
+// Quantizer and product in one call; the codes and their scales are scratch, if they leave the kernel at all.
 Tensor fp8_block_linear(const Tensor& x, const Tensor& weight, const Tensor& weight_scale, const std::optional<Tensor>& bias, bool out_fp16, bool transposed_b,
                         bool e5m2) {
     check_input(x, "x", 16);
@@ -433,11 +433,12 @@ Tensor fp8_block_linear(const Tensor& x, const Tensor& weight, const Tensor& wei
     STD_TORCH_CHECK(x.size(1) == depth, "x's row length must equal the weight axis that is contracted");
     torch::stable::accelerator::DeviceGuard guard(device);
     Tensor c = make_empty({M, transposed_b ? K : N}, half_dtype(out_fp16), device);
-    Tensor scratch = make_empty({M * (depth + 4 * blocks_of(depth))}, aoti_torch_dtype_uint8(), device);   // the codes, then the scales
-    uint8_t* const q = static_cast<uint8_t*>(scratch.mutable_data_ptr());
-    const bool ok = launch_fp8_block_linear(x.const_data_ptr(), q, reinterpret_cast<float*>(q + M * depth), static_cast<const uint8_t*>(weight.const_data_ptr()),
-                                            static_cast<const float*>(weight_scale.const_data_ptr()), bias_ptr(bias),
-                                            static_cast<uint16_t*>(c.mutable_data_ptr()), M, N, K, transposed_b, is_half(x) ? 1 : 0, e5m2 ? 1 : 0,
+    const int64_t bytes = feather_fp8_block_linear_scratch_bytes(M, depth);
+    std::optional<Tensor> scratch;
+    if (bytes > 0) scratch = make_empty({bytes}, aoti_torch_dtype_uint8(), device);
+    const bool ok = launch_fp8_block_linear(x.const_data_ptr(), scratch.has_value() ? scratch->mutable_data_ptr() : nullptr,
+                                            static_cast<const uint8_t*>(weight.const_data_ptr()), static_cast<const float*>(weight_scale.const_data_ptr()),
+                                            bias_ptr(bias), static_cast<uint16_t*>(c.mutable_data_ptr()), M, N, K, transposed_b, is_half(x) ? 1 : 0, e5m2 ? 1 : 0,
                                             weight.scalar_type() == ScalarType::Float8_e5m2 ? 1 : 0, out_fp16 ? 0 : 1, current_stream(device));
     STD_TORCH_CHECK(ok, "fp8_block_linear launch failed");
     return c;

@@ -162,11 +162,13 @@ bool launch_fp8_block_quantize(const void* x, void* q, float* scale, int64_t M, 
 bool launch_fp8_block_mm(const uint8_t* a, const float* a_scale, const uint8_t* w, const float* w_scale, const uint16_t* bias, uint16_t* c, int64_t M,
                          int64_t N, int64_t K, bool transposed_b, int a_e5m2, int w_e5m2, int output_dtype, feather_stream_t stream);
 
-/* launch_fp8_block_quantize of x ([M, K], backward [M, N]) into the caller's q and q_scale, and launch_fp8_block_mm of those, with the
- * weight's first tiles on their way while the quantizer runs. input_fp16: x's type; q_e5m2: the codes'. No counterpart in the reference. */
-bool launch_fp8_block_linear(const void* x, uint8_t* q, float* q_scale, const uint8_t* w, const float* w_scale, const uint16_t* bias, uint16_t* c,
-                             int64_t M, int64_t N, int64_t K, bool transposed_b, int input_fp16, int q_e5m2, int w_e5m2, int output_dtype,
-                             feather_stream_t stream);
+/* Quantizer and product in one call, with the bits of launch_fp8_block_quantize and launch_fp8_block_mm: x is [M, K] (backward [M, N]) in 16
+ * bits (input_fp16), q_e5m2 the codes' type. Up to 8 rows one kernel does both; beyond, the codes and scales go through `scratch`
+ * (feather_fp8_block_linear_scratch_bytes(M, contraction) bytes, 16-byte aligned; NULL where that is 0) and the weight's first tiles are on their
+ * way while the quantizer runs. No counterpart in the reference. */
+bool launch_fp8_block_linear(const void* x, void* scratch, const uint8_t* w, const float* w_scale, const uint16_t* bias, uint16_t* c, int64_t M, int64_t N,
+                             int64_t K, bool transposed_b, int input_fp16, int q_e5m2, int w_e5m2, int output_dtype, feather_stream_t stream);
+int64_t feather_fp8_block_linear_scratch_bytes(int64_t M, int64_t depth);
 
 /* Diagnostic for the block-scaled product's bounded waits, as feather_scaled_mm_status. No counterpart in the reference. */
 int feather_fp8_block_mm_status(uint32_t* out);

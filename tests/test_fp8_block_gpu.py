@@ -145,16 +145,25 @@ def test_product_of_no_rows(cuda_device):
     assert fo.fp8_block_dgrad(torch.empty(0, 256, device=cuda_device, dtype=torch.float16), w, ws).shape == (0, 128)
 
 
-@pytest.mark.parametrize("m", [1, 20, 90, 513])
-def test_linear_and_dgrad_are_the_quantizer_and_the_product(cuda_device, m):
-    n, k = 400, 656
+@pytest.mark.parametrize("n,k", [(400, 656), (272, 4112), (5136, 144), (1040, 2064)])
+@pytest.mark.parametrize("m", [1, 2, 7, 8, 9, 16, 17, 32, 33, 90, 513])
+def test_linear_and_dgrad_are_the_quantizer_and_the_product(cuda_device, m, n, k):
     w, ws = (t.to(cuda_device) for t in fo.quantize_fp8_weight(_rand(n, k, torch.float32, 1, 0.02)))
     x = _rand(m, k, torch.bfloat16, 2).to(cuda_device)
     q, s = fo.quantize_fp8_activation(x)
     assert torch.equal(fo.fp8_block_linear(x.view(1, m, k), w, ws)[0], fo.fp8_block_mm(q, s, w, ws))
+    bias = _rand(1, n, torch.float16, 4)[0].to(cuda_device)
+    q, s = fo.quantize_fp8_activation(x, E5M2)
+    assert torch.equal(fo.fp8_block_linear(x, w, ws, bias, torch.float16, E5M2), fo.fp8_block_mm(q, s, w, ws, bias, torch.float16))
     g = _rand(m, n, torch.float16, 3, 1e-3).to(cuda_device)
     q, s = fo.quantize_fp8_activation(g, E5M2)
     assert torch.equal(fo.fp8_block_dgrad(g, w, ws, torch.float16, E5M2), fo.fp8_block_mm(q, s, w, ws, None, torch.float16, True))
+    g[m // 2, n // 3] = float("inf")   # its row is NaN, and no other
+    g[-1] = 0 if m > 1 else g[-1]
+    out = fo.fp8_block_dgrad(g, w, ws)
+    q, s = fo.quantize_fp8_activation(g)
+    assert torch.equal(out.isnan(), fo.fp8_block_mm(q, s, w, ws, None, torch.bfloat16, True).isnan())
+    assert out.isnan().any(1).nonzero().flatten().tolist() == [r for r in range(m) if not torch.isfinite(g[r]).all()]
 
 
 # --------------------------------------------------------------------------------------------------------------------
@@ -323,6 +332,60 @@ def test_feed_forward_block_captured_and_on_another_stream(cuda_device, m):
     graph.replay()
     for name, value in expected_other.items():
         assert torch.equal(captured[name], value), name
+
+
+def test_products_at_once_on_two_streams(cuda_device):
+    # a small and a pair product that share SMs, over and over: the same bits as alone
+    small, large = _operands(40, 2048, 2064, E4M3, E4M3, False, seed=1), _operands(1500, 1552, 1040, E4M3, E4M3, True, seed=2)
+    expected = fo.fp8_block_mm(*small), fo.fp8_block_mm(*large, transposed_b=True)
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    got = [], []
+    for stream in streams:
+        stream.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        with torch.cuda.stream(streams[0]):
+            got[0].append(fo.fp8_block_mm(*small))
+        with torch.cuda.stream(streams[1]):
+            got[1].append(fo.fp8_block_mm(*large, transposed_b=True))
+    torch.cuda.synchronize()
+    for results, value in zip(got, expected):
+        assert all(torch.equal(r, value) for r in results)
+
+
+def test_offsets_beyond_32_bits(cuda_device):
+    # matrices of more than 2^31 elements; the first, a middle and the last rows against the definitions
+    def inputs(rows, width, seed, size=1.0):
+        g = torch.Generator(device=cuda_device).manual_seed(seed)
+        return torch.randn(rows, width, device=cuda_device, generator=g, dtype=torch.bfloat16) * size
+
+    rows = torch.tensor([0, 70001, 139998, 139999])
+    x = inputs(140000, 16384, 1)
+    q, s = fo.quantize_fp8_activation(x)
+    q_ref, s_ref = ofb.quantize_f32(x[rows].cpu(), E4M3)
+    assert torch.equal(q[rows].cpu().view(torch.uint8), q_ref.view(torch.uint8)) and torch.equal(s[:, rows].cpu(), s_ref)
+    w, ws = (t.to(cuda_device) for t in fo.quantize_fp8_weight(_rand(16, 16384, torch.float32, 2, 0.02)))
+    out = fo.fp8_block_mm(q, s, w, ws)
+    _product_close(out[rows], q[rows], s[:, rows], w, ws, None, False)
+    weight = torch.ones(16384, device=cuda_device, dtype=torch.bfloat16)
+    q, s, _, rstd = fo.rms_norm_quantize_fp8(x, weight)
+    _codes_close(q[rows], s[:, rows], ofb.rms_norm(x[rows].cpu(), weight.cpu(), 1e-6)[0], E4M3, 40 * 2.0**-24)
+    gx, _ = fo.rms_norm_dgrad(x, x, weight, rstd)
+    ref = ofb.rms_norm_grad(x[rows].cpu(), x[rows].cpu(), weight.cpu(), rstd[rows].cpu())
+    assert ((gx[rows].cpu().double() - ref[0]).abs() <= ref[0].abs() * HALF[torch.bfloat16] + ref[2] * 50 * 2.0**-24).all()
+    del gx, q, s
+    gate_up = x.view(70000, 32768)
+    rows = torch.tensor([0, 35001, 69999])
+    q, s = fo.silu_mul_quantize_fp8(gate_up)
+    _codes_close(q[rows], s[:, rows], ofb.silu_mul(gate_up[rows].cpu()), E4M3, 30 * 2.0**-23)
+    out = fo.silu_mul_dgrad(x.view(-1)[: 70000 * 16384].view(70000, 16384), gate_up)
+    ref = ofb.silu_mul_grad(x.view(-1)[: 70000 * 16384].view(70000, 16384)[rows].cpu(), gate_up[rows].cpu())
+    assert ((out[rows].cpu().double() - ref).abs() <= ref.abs() * HALF[torch.bfloat16] + 1e-4).all()
+    del out, q, s, x, gate_up
+    # an output of more than 2^31 elements
+    rows = torch.tensor([0, 70001, 139999])
+    q, s, w, ws = _operands(140000, 16384, 128, E4M3, E4M3, False)
+    out = fo.fp8_block_mm(q, s, w, ws)
+    _product_close(out[rows], q[rows], s[:, rows], w, ws, None, False)
 
 
 def test_compiled_caller(cuda_device):
