@@ -373,6 +373,83 @@ __global__ void __launch_bounds__(kThreads) rms_norm_dgrad_kernel(const NormGrad
     }
 }
 
+// The same for few rows, in one launch and without partials: `rstd` is given, so dw needs nothing of a row but its values. The first M
+// CTAs have a row each and write dx, the others 64 channels each and add grad n over the rows: 8 threads abreast, blockDim.x / 8 rows at a
+// time, then the lanes and the warps in order. The inputs are read twice, the second time from L2. At 333 x 2576 a call costs the host
+// 8 us instead of 11.5, and the device less too.
+constexpr int kFewRows = 512;
+constexpr int kFewWidth = kMaxNormThreads * kVec;   // one chunk per thread
+constexpr int kFewThreads = 256;                    // at least, for the channels' CTAs
+constexpr int kColumnTile = 64;
+
+template <bool kFp16, bool kWeightF32>
+__global__ void __launch_bounds__(kMaxNormThreads) rms_norm_dgrad_few_kernel(const NormGradParams p, float* __restrict__ grad_weight) {
+    __shared__ float slots[32];
+    __shared__ float2 sums[32][kColumnTile / 2];
+    start_after_kernel_ahead();
+    const int width = static_cast<int>(p.K);
+    const int rows = static_cast<int>(p.M);
+    if (static_cast<int>(blockIdx.x) < rows) {
+        const int64_t row = blockIdx.x;
+        const int column = threadIdx.x * kVec;
+        const bool live = column < width;
+        const float rstd = __ldg(p.rstd + row);
+        Pairs n = {}, u = {}, r = {};
+        float2 dots = both(0.0f);
+        if (live) {
+            Pairs w;
+            unpack8<kFp16>(load16(p.x + row * p.K + column), n);
+            unpack8<kFp16>(load16(p.grad + row * p.K + column), u);
+            if (p.grad_residual != nullptr) unpack8<kFp16>(load16(p.grad_residual + row * p.K + column), r);
+            load_weight<kFp16, kWeightF32>(p.weight, column, w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                n[i] = __fmul2_rn(n[i], both(rstd));
+                u[i] = __fmul2_rn(u[i], w[i]);
+                dots = __ffma2_rn(u[i], n[i], dots);
+            }
+        }
+        const float2 back = both(-rstd * (row_sum(dots.x + dots.y, slots) / static_cast<float>(width)));
+        if (live) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = __ffma2_rn(n[i], back, __ffma2_rn(u[i], both(rstd), r[i]));
+            *reinterpret_cast<uint4*>(p.grad_x + row * p.K + column) = pack8<kFp16>(r);
+        }
+        return;
+    }
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int column = (blockIdx.x - rows) * kColumnTile + lane % 8 * kVec;
+    Pairs sum = {};
+    if (column < width) {
+#pragma unroll 4
+        for (int row = threadIdx.x / 8; row < rows; row += blockDim.x / 8) {
+            Pairs n, g;
+            unpack8<kFp16>(load16(p.x + static_cast<int64_t>(row) * p.K + column), n);
+            unpack8<kFp16>(load16(p.grad + static_cast<int64_t>(row) * p.K + column), g);
+            const float2 rstd = both(__ldg(p.rstd + row));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[i] = __ffma2_rn(g[i], __fmul2_rn(n[i], rstd), sum[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int step = 8; step < 32; step <<= 1) {
+            sum[i].x += __shfl_xor_sync(0xffffffffu, sum[i].x, step);
+            sum[i].y += __shfl_xor_sync(0xffffffffu, sum[i].y, step);
+        }
+        if (lane < 8) sums[warp][lane * 4 + i] = sum[i];
+    }
+    __syncthreads();
+    const int pair = threadIdx.x;
+    const int first = (blockIdx.x - rows) * kColumnTile + 2 * pair;
+    if (pair < kColumnTile / 2 && first < width) {
+        float2 total = sums[0][pair];
+        for (int w = 1; w < static_cast<int>(blockDim.x >> 5); ++w) total = __fadd2_rn(total, sums[w][pair]);
+        *reinterpret_cast<float2*>(grad_weight + first) = total;
+    }
+}
+
 // out[k] = sum over the rows of partials, row groups first (one per warp), then the groups in order.
 constexpr int kSumWarps = 8;
 __global__ void __launch_bounds__(32 * kSumWarps) column_sum_kernel(const float* __restrict__ partials, float* __restrict__ out, int rows, int64_t K) {
@@ -474,8 +551,15 @@ bool launch_norm(const NormParams& p, cudaStream_t stream) {
     return launch_kernel(kernel, (p.M + rows - 1) / rows, dim3(shape.threads, shape.rows), 0, stream, true, p);
 }
 
+bool few_rows(int64_t M, int64_t K) { return M <= kFewRows && K <= kFewWidth; }
+
 template <bool kFp16, bool kWeightF32>
 bool launch_norm_grad(const NormGradParams& p, float* grad_weight, cudaStream_t stream) {
+    if (few_rows(p.M, p.K)) {
+        const int threads = static_cast<int>((p.K / kVec + 31) / 32 * 32);
+        return launch_kernel(rms_norm_dgrad_few_kernel<kFp16, kWeightF32>, p.M + (p.K + kColumnTile - 1) / kColumnTile,
+                             dim3(threads < kFewThreads ? kFewThreads : threads), 0, stream, true, p, grad_weight);
+    }
     const RowShape shape = row_shape(p.M, p.K);
     const int grid = norm_grad_grid(p.M, shape);
     const auto kernel = shape.chunks == 1   ? rms_norm_dgrad_kernel<kFp16, kWeightF32, 1, kMaxNormThreads>
@@ -546,15 +630,15 @@ extern "C" bool launch_rms_norm_fp8(const void* x, const void* residual, const v
 }
 
 extern "C" int64_t feather_rms_norm_dgrad_partial_floats(int64_t M, int64_t K) {
-    if (M <= 0 || K <= 0 || K > kMaxNormWidth) return 0;
+    if (M <= 0 || K <= 0 || K > kMaxNormWidth || few_rows(M, K)) return 0;
     return norm_grad_grid(M, row_shape(M, K)) * K;
 }
 
 extern "C" bool launch_rms_norm_dgrad(const void* grad, const void* x, const void* weight, const float* rstd, const void* grad_residual, void* grad_x,
                                       float* grad_weight, float* partials, int64_t M, int64_t K, int input_fp16, int weight_f32, cudaStream_t stream) {
     if (M <= 0 || M > 0x7fffffff || K <= 0 || K % 16 != 0 || K > kMaxNormWidth) return false;
-    if (grad == nullptr || x == nullptr || weight == nullptr || rstd == nullptr || grad_x == nullptr || grad_weight == nullptr || partials == nullptr) return false;
-    if (!aligned(grad, 16) || !aligned(x, 16) || !aligned(weight, 16) || !aligned(grad_residual, 16) || !aligned(grad_x, 16) || !aligned(partials, 16)) return false;
+    if (grad == nullptr || x == nullptr || weight == nullptr || rstd == nullptr || grad_x == nullptr || grad_weight == nullptr || (partials == nullptr && !few_rows(M, K))) return false;
+    if (!aligned(grad, 16) || !aligned(x, 16) || !aligned(weight, 16) || !aligned(grad_residual, 16) || !aligned(grad_x, 16) || !aligned(grad_weight, 8) || !aligned(partials, 16)) return false;
     const NormGradParams p{static_cast<const uint16_t*>(grad), static_cast<const uint16_t*>(x), weight, rstd, static_cast<const uint16_t*>(grad_residual),
                            static_cast<uint16_t*>(grad_x), partials, M, K};
     

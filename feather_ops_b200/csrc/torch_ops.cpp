@@ -491,10 +491,13 @@ std::tuple<Tensor, Tensor> rms_norm_dgrad(const Tensor& grad, const Tensor& x, c
     torch::stable::accelerator::DeviceGuard guard(device);
     Tensor grad_x = make_empty({M, K}, half_dtype(is_half(x)), device);
     Tensor grad_weight = make_empty({K}, aoti_torch_dtype_float32(), device);
-    Tensor partials = make_empty({feather_rms_norm_dgrad_partial_floats(M, K)}, aoti_torch_dtype_float32(), device);
+    const int64_t floats = feather_rms_norm_dgrad_partial_floats(M, K);
+    std::optional<Tensor> partials;
+    if (floats > 0) partials = make_empty({floats}, aoti_torch_dtype_float32(), device);
     const bool ok = launch_rms_norm_dgrad(grad.const_data_ptr(), x.const_data_ptr(), weight.const_data_ptr(), static_cast<const float*>(rstd.const_data_ptr()),
                                           grad_residual.has_value() ? grad_residual->const_data_ptr() : nullptr, grad_x.mutable_data_ptr(),
-                                          static_cast<float*>(grad_weight.mutable_data_ptr()), static_cast<float*>(partials.mutable_data_ptr()), M, K,
+                                          static_cast<float*>(grad_weight.mutable_data_ptr()),
+                                          partials.has_value() ? static_cast<float*>(partials->mutable_data_ptr()) : nullptr, M, K,
                                           is_half(x) ? 1 : 0, weight.scalar_type() == ScalarType::Float ? 1 : 0, current_stream(device));
     STD_TORCH_CHECK(ok, "rms_norm_dgrad launch failed");
     return std::make_tuple(std::move(grad_x), std::move(grad_weight));

@@ -182,8 +182,8 @@ bool launch_rms_norm_fp8(const void* x, const void* residual, const void* weight
 
 /* Backward pass of the norm: with n = x rstd (x: what the norm was taken of, i.e. residual_out where there was a residual) and
  * u = grad * weight, grad_x = rstd (u - n mean(u n)) + grad_residual, grad_weight = sum over rows of grad * n (float32, the same bits on
- * every run of one device). grad_residual: [M, K] or NULL. partials: feather_rms_norm_dgrad_partial_floats(M, K) floats of scratch, 16-byte
- * aligned. M >= 1, the norm's other conditions. No counterpart in the reference. */
+ * every run of one device). grad_residual: [M, K] or NULL. grad_weight is 8-byte aligned. partials: feather_rms_norm_dgrad_partial_floats(M, K)
+ * floats of scratch, 16-byte aligned (NULL where that is 0, with few rows). M >= 1, the norm's other conditions. No counterpart in the reference. */
 bool launch_rms_norm_dgrad(const void* grad, const void* x, const void* weight, const float* rstd, const void* grad_residual, void* grad_x,
                            float* grad_weight, float* partials, int64_t M, int64_t K, int input_fp16, int weight_f32, feather_stream_t stream);
 int64_t feather_rms_norm_dgrad_partial_floats(int64_t M, int64_t K);
