@@ -995,52 +995,58 @@ bool launch_pair(const Args& args) {
     return cudaLaunchKernelEx(&config, kernel, map_a, map_w, map_c, p) == cudaSuccess;
 }
 
-// Microseconds that a product takes on the small kernel with T tokens per tile and `splits` K splits, or a negative number
-// where the clusters would not be resident at once. Per launch 3.5; per k block of a CTA 0.29 with 16 or 32 tokens and 0.45 with
-// 128 (every SM busy; the activation tile then is as large as the weight's); the exchange of the partial sums 1.0 and 1.8.
+// What a product is expected to cost, in microseconds, and the K splits that give it. Fitted to single launches over weights in HBM
+// (M 1 .. 3600, N 512 .. 12288, K 512 .. 4096): a launch 0.6, a round of CTAs its start and end and a time per k block, the exchange of
+// the partial sums of a split.
+struct Choice {
+    double cost;
+    int splits;
+};
+
 template <int T, bool kBackward, bool kOutBf16, bool kQuantize>
-double small_cost(const Args& args, int splits) {
+Choice small_choice(const Args& args) {
+    constexpr double kRound = T == 16 ? 2.6 : T == 32 ? 2.8 : 5.0;
+    constexpr double kPerBlock = T == 16 ? 0.29 : T == 32 ? 0.36 : 0.37;
+    constexpr double kExchange = T == 16 ? 2.0 : 1.8;
     const int64_t num_kb = (args.depth() + kBlock - 1) / kBlock;
     const int64_t tiles = (args.M + T - 1) / T * ((args.width() + 127) / 128);
-    const int clusters = splits > num_kb ? 0 : small_clusters<T, kBackward, kOutBf16, kQuantize>(splits);
-    if (clusters <= 0 || (splits > 1 && tiles > clusters)) return -1.0;
-    const double rounds = static_cast<double>((tiles + clusters - 1) / clusters);
-    return 3.5 + rounds * static_cast<double>((num_kb + splits - 1) / splits) * (T == 128 ? 0.45 : 0.29) + (splits == 1 ? 0.0 : T == 128 ? 1.8 : 1.0);
+    Choice best{1e30, 1};
+    for (int splits = 1; splits <= kMaxSplits && splits <= num_kb; ++splits) {
+        const int clusters = small_clusters<T, kBackward, kOutBf16, kQuantize>(splits);
+        if (clusters <= 0 || (splits > 1 && tiles > clusters)) continue;   // a split pays only where all clusters are resident at once
+        const double rounds = static_cast<double>((tiles + clusters - 1) / clusters);
+        const double blocks = static_cast<double>((num_kb + splits - 1) / splits);
+        const double cost = 0.6 + rounds * (kRound + kPerBlock * blocks) + (splits == 1 ? 0.0 : kExchange);
+        if (cost < best.cost) best = {cost, splits};
+    }
+    return best;
 }
 
-template <int T, bool kBackward, bool kOutBf16, bool kQuantize>
-bool launch_best_small(const Args& args, double pair_cost) {
-    int best = 1;
-    double best_cost = small_cost<T, kBackward, kOutBf16, kQuantize>(args, 1);
-    for (int splits = 2; splits <= kMaxSplits; ++splits) {
-        const double cost = small_cost<T, kBackward, kOutBf16, kQuantize>(args, splits);
-        if (cost >= 0.0 && cost < best_cost) {
-            best = splits;
-            best_cost = cost;
-        }
-    }
-    if constexpr (T == 128) {
-        if (best_cost > pair_cost) return launch_pair<kBackward, kOutBf16>(args);
-    }
-    return launch_small<T, kBackward, kOutBf16, kQuantize>(args, best);
-}
-
-// Up to 16 and 32 tokens their own tiles, above that 128 tokens per tile or the pair kernel, whichever the model says: a round of the
-// pair kernel's tiles costs 0.57 us per k block and 1 us for its end (512 x 4096 x 4096: 17.7 us small, 21.1 pair; 1024 x 4096 x 4096:
-// 33.7 against 22.2; 777 x 3856 x 2576: 26.6 against 16.3; 300 x 12288 x 4096: 33.8 against 37.5).
-template <bool kBackward, bool kOutBf16>
-bool launch(const Args& args) {
-    constexpr double kNever = 1e30;
-    if (args.x != nullptr) {
-        return launch_best_small<16, kBackward, kOutBf16, true>(args, kNever);
-    }
-    if (args.M <= 16) return launch_best_small<16, kBackward, kOutBf16, false>(args, kNever);
-    if (args.M <= 32) return launch_best_small<32, kBackward, kOutBf16, false>(args, kNever);
-    const int pairs = device_info().sm_count / 2;
+// A round of the pair kernel's tiles, 0.46 a k block.
+double pair_cost(const Args& args) {
+    const int64_t pairs = device_info().sm_count / 2;
     const int64_t tiles = (args.M + 255) / 256 * ((args.width() + kPairN - 1) / kPairN);
     const int64_t num_kb = (args.depth() + kBlock - 1) / kBlock;
-    const double pair_cost = 4.0 + static_cast<double>((tiles + pairs - 1) / pairs) * (0.57 * static_cast<double>(num_kb) + 1.0);
-    return launch_best_small<128, kBackward, kOutBf16, false>(args, pair_cost);
+    return 4.2 + static_cast<double>((tiles + pairs - 1) / pairs) * (1.3 + 0.46 * static_cast<double>(num_kb));
+}
+
+// Up to 16 tokens one tile of 16. Above, the cheapest of tiles of 32 (up to 128 tokens), tiles of 128 and the pair kernel. Measured (us): 78 x 6016 x
+// 640 5.2 with tiles of 32 and 6.0 of 128, 64 x 5120 x 5120 13.5 and 10.9; 512 x 4096 x 4096 15.8 with tiles of 128 and 21.1 on the pair kernel,
+// 744 x 7872 x 560 22.0 and 12.6, 1024 x 4096 x 4096 33.7 and 22.2.
+template <bool kBackward, bool kOutBf16>
+bool launch(const Args& args) {
+    if (args.x != nullptr) return launch_small<16, kBackward, kOutBf16, true>(args, small_choice<16, kBackward, kOutBf16, true>(args).splits);
+    if (args.M <= 16) return launch_small<16, kBackward, kOutBf16, false>(args, small_choice<16, kBackward, kOutBf16, false>(args).splits);
+    Choice narrow{1e30, 1}, wide{1e30, 1};
+    double pair = 1e30;
+    if (args.M <= 128) narrow = small_choice<32, kBackward, kOutBf16, false>(args);
+    if (args.M > 32) {
+        wide = small_choice<128, kBackward, kOutBf16, false>(args);
+        pair = pair_cost(args);
+    }
+    if (narrow.cost <= wide.cost && narrow.cost <= pair) return launch_small<32, kBackward, kOutBf16, false>(args, narrow.splits);
+    if (wide.cost <= pair) return launch_small<128, kBackward, kOutBf16, false>(args, wide.splits);
+    return launch_pair<kBackward, kOutBf16>(args);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -169,7 +169,7 @@ def test_linear_and_dgrad_are_the_quantizer_and_the_product(cuda_device, m, n, k
 # --------------------------------------------------------------------------------------------------------------------
 # Norm
 # --------------------------------------------------------------------------------------------------------------------
-NORM_SHAPES = [(512, 16), (513, 1040), (512, 8208), (1, 16), (1, 5120), (2, 32768), (3, 272), (7, 128), (33, 8192), (300, 2576), (333, 2576), (601, 4096), (1500, 144), (700, 16400)]
+NORM_SHAPES = [(512, 16), (513, 272), (1024, 1040), (1025, 528), (512, 8208), (1, 16), (1, 5120), (2, 32768), (3, 272), (7, 128), (33, 8192), (300, 2576), (333, 2576), (601, 4096), (1500, 144), (700, 16400)]
 
 
 @pytest.mark.parametrize("residual", [False, True], ids=["plain", "residual"])
