@@ -516,17 +516,17 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
 // core once per 128-deep block. So a k block's product is two UMMA groups of half the tile's outputs (h = 0, 1: rows
 // h * seg .. of both CTAs' weight boxes), each with two accumulators, barriers and four epilogue warps of its own: the warps of one
 // half load accumulators from tensor memory while those of the other scale theirs.
-constexpr int kPairStages = 6;
+constexpr int kPairStages = 4;
 constexpr int kPairN = 256;
 constexpr int kPairEpilogueWarps = 8;                              // [half][lane quarter]
-constexpr int kPairThreads = 32 * (4 + kPairEpilogueWarps);        // warps 0-3: load, multiply, relay, scales
+constexpr int kPairThreads = 32 * (4 + kPairEpilogueWarps);        // warps 0-3: load, multiply h = 0 and 1, scales
 constexpr int kImageBytes = 32 * 64;                               // 32 rows x 32 outputs of 16 bits
 
 struct PairSmem {
     static constexpr int kStageBytes = 2 * kTileBytes;             // this CTA's 128 activation rows and its half of the outputs
-    static constexpr int kImageOff = kPairStages * kStageBytes;    // one image per epilogue warp
+    static constexpr int kImageOff = kPairStages * kStageBytes;    // [epilogue warp][4 chunks]
     static constexpr int kRaw = 132;                               // floats: 128 row scales, two of the weight's, padding
-    static constexpr int kRawOff = kImageOff + kPairEpilogueWarps * kImageBytes;
+    static constexpr int kRawOff = kImageOff + kPairEpilogueWarps * 4 * kImageBytes;
     static constexpr int kScaleOff = kRawOff + kScaleRing * kRaw * 4;   // products [4 k blocks][2 weight blocks][128 rows]
     static constexpr int kBarOff = kScaleOff + 4 * 2 * 128 * 4;
     static constexpr int kNumBars = 3 * kPairStages + 8;
@@ -541,9 +541,9 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     using L = PairSmem;
     extern __shared__ uint8_t smem_dyn[];
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~static_cast<uintptr_t>(1023));
-    uint64_t* const load_full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);   // this CTA's boxes have landed
-    uint64_t* const load_empty = load_full + kPairStages;                         // signalled in both CTAs by CTA 0's commits
-    uint64_t* const both_full = load_empty + kPairStages;                         // CTA 0 only: both CTAs' boxes have landed
+    uint64_t* const load_full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);   // CTA 1: its boxes have landed
+    uint64_t* const load_empty = load_full + kPairStages;                         // signalled in both CTAs by the commits of both halves
+    uint64_t* const both_full = load_empty + kPairStages;                         // CTA 0: its own boxes have landed, and CTA 1's
     uint64_t* const tmem_full = both_full + kPairStages;                          // [half][accumulator]
     uint64_t* const tmem_empty = tmem_full + 4;                                   // CTA 0 only
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(load_full + L::kNumBars);
@@ -557,7 +557,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         *abort_flag = 0u;
         for (int s = 0; s < kPairStages; ++s) {
             mbar_init(&load_full[s], 1);
-            mbar_init(&load_empty[s], 1);
+            mbar_init(&load_empty[s], 2);
             mbar_init(&both_full[s], 2);
         }
         for (int s = 0; s < 4; ++s) {
@@ -602,41 +602,40 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     ok = guard.wait(&load_empty[slot.idx], slot.phase ^ 1u, kSiteLoadEmpty);
                     if (!ok) break;
                     uint8_t* const stage = smem + slot.idx * L::kStageBytes;
-                    mbar_arrive_expect_tx(&load_full[slot.idx], stage_bytes);
-                    tma_load_2d(stage, &map_a, &load_full[slot.idx], kb * kBlock, m0);
-                    tma_load_2d(stage + kTileBytes, &map_w, &load_full[slot.idx], kBackward ? n0 : kb * kBlock, kBackward ? kb * kBlock : n0);
+                    uint64_t* const landed = cta == 0 ? &both_full[slot.idx] : &load_full[slot.idx];
+                    mbar_arrive_expect_tx(landed, stage_bytes);
+                    tma_load_2d(stage, &map_a, landed, kb * kBlock, m0);
+                    tma_load_2d(stage + kTileBytes, &map_w, landed, kBackward ? n0 : kb * kBlock, kBackward ? kb * kBlock : n0);
                     slot.advance(kPairStages);
                 }
             }
-        } else if (warp == 1 && cta == 0 && elect_one()) {
-            // ------------------------------------------------------------------ UMMA issuer of the pair
+        } else if ((warp == 1 || warp == 2) && cta == 0 && elect_one()) {
+            // ------------------------------------------------------------------ UMMA issuers of the pair, one per half of the outputs. A wait,
+            // even on a barrier that is there, takes the issuing thread 75 clocks and a group with its commits 200: one thread for both
+            // halves was the slowest part of the loop (646 clocks a k block, 512 of the tensor core).
+            const int h = warp - 1;
             Ring slot, out;
             bool ok = true;
             for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
                 for (int kb = 0; kb < p.num_kb; ++kb) {
+                    // backward the weight box is MN-major: the group's outputs are bytes h * seg .. of its 128-byte rows
                     const uint32_t a_addr = smem_u32(smem + slot.idx * L::kStageBytes);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (h == 0) ok = guard.wait(&both_full[slot.idx], slot.phase, kSiteOperandFull);
-                        ok = ok && guard.wait(&tmem_empty[2 * h + out.idx], out.phase ^ 1u, kSiteTmemEmpty);
-                        if (!ok) break;
-                        tc_fence_after_sync();
-                        // backward the weight box is MN-major: the group's outputs are bytes h * seg .. of its 128-byte rows
-                        const uint32_t w_addr = a_addr + kTileBytes + h * (kBackward ? seg : seg * 128);
-#pragma unroll
-                        for (int k = 0; k < kBlock / 32; ++k) {
-                            const uint64_t desc_w = kBackward ? make_desc_sw128_mnmajor(w_addr + k * 32 * 128) : make_desc_sw128_kmajor(w_addr + k * 32);
-                            umma_f8_pair(tmem_base + out.idx * kPairN + h * kPairN / 2, make_desc_sw128_kmajor(a_addr + k * 32), desc_w, p.idesc, k != 0 ? 1u : 0u);
-                        }
-                        umma_commit_pair_both(&tmem_full[2 * h + out.idx]);
-                    }
+                    const uint32_t w_addr = a_addr + kTileBytes + h * (kBackward ? seg : seg * 128);
+                    ok = guard.wait(&both_full[slot.idx], slot.phase, kSiteOperandFull) && guard.wait(&tmem_empty[2 * h + out.idx], out.phase ^ 1u, kSiteTmemEmpty);
                     if (!ok) break;
+                    tc_fence_after_sync();
+#pragma unroll
+                    for (int k = 0; k < kBlock / 32; ++k) {
+                        const uint64_t desc_w = kBackward ? make_desc_sw128_mnmajor(w_addr + k * 32 * 128) : make_desc_sw128_kmajor(w_addr + k * 32);
+                        umma_f8_pair(tmem_base + out.idx * kPairN + h * kPairN / 2, make_desc_sw128_kmajor(a_addr + k * 32), desc_w, p.idesc, k != 0 ? 1u : 0u);
+                    }
+                    umma_commit_pair_both(&tmem_full[2 * h + out.idx]);
                     umma_commit_pair_both(&load_empty[slot.idx]);
                     slot.advance(kPairStages);
                     out.advance(2);
                 }
             }
-        } else if (warp == 2 && elect_one()) {
+        } else if (warp == 1 && cta == 1 && elect_one()) {
             // ------------------------------------------------------------------ tells CTA 0 that this CTA's boxes have landed
             Ring slot;
             bool ok = true;
@@ -719,11 +718,12 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         const int half = (warp - 4) / 4;
         constexpr int kChunks = 2 * seg / 32;   // of 32 outputs: those of CTA 0's weight rows, then CTA 1's
         const int twist = (lane >> 1) & 3;   // 64-byte swizzle: the 16-byte chunk index is XORed with bits 7-8 of the address
-        uint8_t* const image = smem + L::kImageOff + (warp - 4) * kImageBytes;
+        uint8_t* const images = smem + L::kImageOff + (warp - 4) * kChunks * kImageBytes;
+        // the outputs of CTA 0's weight rows come first, then CTA 1's
+        const auto chunk_column = [&](int col0, int c) { return col0 + half * seg + (2 * c >= kChunks ? half_n + (c - kChunks / 2) * 32 : c * 32); };
         const float* const products = reinterpret_cast<const float*>(smem + L::kScaleOff) + quarter * 32 + lane;
         const uint32_t empty0 = map_to_cta(smem_u32(tmem_empty + 2 * half), 0);
         const uint32_t taddr0 = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + half * (kPairN / 2);
-        bool stored = false;
         uint32_t turn = 0;   // k blocks so far: their accumulators alternate
         bool ok = true;
         grid_dependency_wait();   // the kernel before this one may still read what this one writes
@@ -770,12 +770,14 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 for (int j = 0; j < 16; ++j) fma2(acc[kChunks - 1][j], v[1][2 * j], v[1][2 * j + 1], s1, s1);
             }
             if (!ok) break;
+            // Output: an image per chunk, so that the warp waits for nothing but the last tile's stores, long done. (With one image per warp
+            // the end of a tile held the tensor core up for 3000 clocks.)
+            if (lane == 0) tma_store_wait_read<0>();
+            __syncwarp();
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
-                const bool other = 2 * c >= kChunks;   // CTA 1's weight rows
-                const int column = col0 + half * seg + (other ? half_n + (c - kChunks / 2) * 32 : c * 32);
-                if (column >= p.width || row0 >= p.M) continue;
-                if (p.bias != nullptr) {
+                const int column = chunk_column(col0, c);
+                if (p.bias != nullptr && column < p.width) {
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
                         if (column + 2 * j < p.width) {
@@ -784,24 +786,24 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                         }
                     }
                 }
-                if (stored) {   // the image's earlier store has been read
-                    if (lane == 0) tma_store_wait_read<0>();
-                    __syncwarp();
-                }
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     const float2* const f = acc[c] + g * 4;
-                    *reinterpret_cast<uint4*>(image + lane * 64 + ((g ^ twist) << 4)) =
+                    *reinterpret_cast<uint4*>(images + c * kImageBytes + lane * 64 + ((g ^ twist) << 4)) =
                         make_uint4(pack_out<kOutBf16>(f[0].x, f[0].y), pack_out<kOutBf16>(f[1].x, f[1].y), pack_out<kOutBf16>(f[2].x, f[2].y), pack_out<kOutBf16>(f[3].x, f[3].y));
                 }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    tma_store_2d(&map_c, image, column, row0);   // clipped at M and width
-                    tma_store_commit();
-                }
-                stored = true;
             }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && row0 < p.M) {
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c) {
+                    const int column = chunk_column(col0, c);
+                    if (column < p.width) tma_store_2d(&map_c, images + c * kImageBytes, column, row0);   // clipped at M and width
+                }
+                tma_store_commit();
+            }
+            __syncwarp();
         }
         if (lane == 0) tma_store_wait<0>();
         __syncwarp();
