@@ -2,7 +2,8 @@
 
 Same Python surface as the reference package (`feather_ops/__init__.py:18-31` there): `scaled_mm_hip`,
 the int8 ConvRot functions and the 3x3 conv, all running hand-written tcgen05 kernels through
-`torch.ops.feather_ops.*`. Importing the package loads the native extension and fails loudly when it has
+`torch.ops.feather_ops.*`. Beside them, without a counterpart in the reference: block-scaled fp8 linears with the RMS norm
+and the gate that write their inputs (`fp8_block`). Importing the package loads the native extension and fails loudly when it has
 not been built: there is no CPU or eager fallback for the kernels.
 """
 
@@ -15,7 +16,7 @@ import torch  # noqa: F401  the extension links against libtorch, so torch has t
 _BUILDING = "feather_ops_b200._build" in getattr(sys, "orig_argv", [])
 
 try:
-    from . import _C  # noqa: F401  registers torch.ops.feather_ops.{scaled_mm,int8_scaled_mm,convrot_quantize,conv2d_3x3}
+    from . import _C  # noqa: F401  registers torch.ops.feather_ops.{scaled_mm,int8_scaled_mm,convrot_quantize,conv2d_3x3,...}
 except ImportError as exc:  # pragma: no cover - depends on the build state
     if not _BUILDING:
         raise ImportError(

@@ -1,6 +1,6 @@
 """Per-operator measurements: every operator of the library at its benchmark shapes, with vendor-library comparators.
 
-    python -m feather_ops_b200.benchmarks [scaled_mm] [msweep] [int8] [conv] [grid] [cells] [--profile] [--peaks FILE]
+    python -m feather_ops_b200.benchmarks [scaled_mm] [msweep] [int8] [conv] [grid] [fp8_block] [cells] [--profile] [--peaks FILE]
 
 `--peaks FILE` names a JSON file with the measured peaks of the device (`hbm_gbs`, `bf16_tflops`); without it only
 the fractions of the nominal peaks are reported. `--profile` is for runs under a profiler: every case makes three
@@ -42,7 +42,7 @@ def wait_records() -> dict:
     from . import _lib
 
     found = {}
-    for symbol in ("feather_scaled_mm_status", "feather_int8_mm_status", "feather_conv3x3_status"):
+    for symbol in ("feather_scaled_mm_status", "feather_int8_mm_status", "feather_conv3x3_status", "feather_fp8_block_mm_status"):
         site, block = _lib.read_status(symbol)
         if site or block:
             found[symbol] = [site, block]
@@ -493,7 +493,57 @@ def bench_cells(device, peaks, groups=None) -> list[dict]:
     return out
 
 
-GROUPS = {"scaled_mm": bench_scaled_mm, "msweep": bench_msweep, "int8": bench_int8, "conv": bench_conv, "grid": bench_grid, "cells": bench_cells}
+# ------------------------------------------------------------------------------------------------------------- fp8_block
+# (tokens, N, K) of a product; the row-wise operators run on (rows, width)
+FP8_BLOCK_PRODUCTS = [(1, 12288, 4096), (24, 5120, 5120), (512, 4096, 4096), (1024, 4096, 4096), (4096, 4096, 4096), (8192, 12288, 4096)]
+FP8_BLOCK_ROWS = [(1, 4096), (333, 2576), (8192, 4096)]
+FP8_BLOCK_GATES = [(1, 12288), (4096, 12288)]
+
+
+def bench_fp8_block(device, peaks) -> list[dict]:
+    from . import fp8_block as fb
+
+    peaks = dict(peaks)
+    if "bf16_tflops" in peaks:
+        peaks["int8_tops"] = 2 * peaks["bf16_tflops"]   # 8-bit products run at twice the 16-bit rate
+    records = []
+
+    def rows_of(m, k):
+        return torch.randn((m, k), device=device).to(torch.bfloat16)
+
+    def case(name, launch, sets, algorithmic_bytes, flop=None, bound="hbm"):
+        timing = time_launches(launch, sets)
+        records.append(_rates({"case": name, "cold": True}, timing, flop=flop, algorithmic_bytes=algorithmic_bytes, bound=bound, peaks=peaks, int8=flop is not None))
+
+    for m, n, k in FP8_BLOCK_PRODUCTS:
+        flop, traffic = 2.0 * m * n * k, n * k + m * k + 2 * m * n
+        bound = "tensor" if flop / NOMINAL["int8_tops"] / 1e3 > traffic / NOMINAL["hbm_gbs"] else "hbm"
+        sets = sets_for(traffic, True)
+        weights = [fb.quantize_fp8_weight(torch.randn((n, k), device=device) * 0.02) for _ in range(sets)]
+        inputs = [rows_of(m, k) for _ in range(sets)]
+        codes = [fb.quantize_fp8_activation(x) for x in inputs]
+        grads = [fb.quantize_fp8_activation(rows_of(m, n)) for _ in range(sets)]
+        case(f"fp8_block_mm {m}x{n}x{k}", lambda i: fb.fp8_block_mm(*codes[i % sets], *weights[i % sets]), sets, traffic, flop, bound)
+        case(f"fp8_block_mm transposed {m}x{n}x{k}", lambda i: fb.fp8_block_mm(*grads[i % sets], *weights[i % sets], transposed_b=True), sets,
+             n * k + m * n + 2 * m * k, flop, bound)
+        case(f"fp8_block_linear {m}x{n}x{k}", lambda i: fb.fp8_block_linear(inputs[i % sets], *weights[i % sets]), sets, traffic + m * k, flop, bound)
+        del weights, inputs, codes, grads
+    for m, k in FP8_BLOCK_ROWS:
+        sets = sets_for(7 * m * k, True)
+        x, r, w = [rows_of(m, k) for _ in range(sets)], [rows_of(m, k) for _ in range(sets)], rows_of(1, k)[0]
+        rstd = torch.ones(m, device=device)
+        case(f"quantize_fp8_activation {m}x{k}", lambda i: fb.quantize_fp8_activation(x[i % sets]), sets, 3 * m * k)
+        case(f"rms_norm_quantize_fp8 residual {m}x{k}", lambda i: fb.rms_norm_quantize_fp8(x[i % sets], w, r[i % sets]), sets, 7 * m * k)
+        case(f"rms_norm_dgrad residual {m}x{k}", lambda i: fb.rms_norm_dgrad(x[i % sets], r[i % sets], w, rstd, x[(i + 1) % sets]), sets, 8 * m * k)
+    for m, f in FP8_BLOCK_GATES:
+        sets = sets_for(5 * m * f, True)
+        gate_up, g = [rows_of(m, 2 * f) for _ in range(sets)], [rows_of(m, f) for _ in range(sets)]
+        case(f"silu_mul_quantize_fp8 {m}x{f}", lambda i: fb.silu_mul_quantize_fp8(gate_up[i % sets]), sets, 5 * m * f)
+        case(f"silu_mul_dgrad {m}x{f}", lambda i: fb.silu_mul_dgrad(g[i % sets], gate_up[i % sets]), sets, 10 * m * f)
+    return records
+
+
+GROUPS = {"scaled_mm": bench_scaled_mm, "msweep": bench_msweep, "int8": bench_int8, "conv": bench_conv, "grid": bench_grid, "fp8_block": bench_fp8_block, "cells": bench_cells}
 
 
 def main(argv):

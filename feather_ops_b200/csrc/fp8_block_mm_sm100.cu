@@ -8,11 +8,13 @@
 // The copy engine's boxes of the row-major weight are operands as they land: 128 bytes along K are a K-major row forward,
 // and backward, where the contraction runs over the weight's rows, the same box is an MN-major operand.
 //
-// Two kernels, picked by `plan`:
+// Two kernels, picked by `launch`:
 //   * small_kernel: 128 outputs x 16, 32 or 128 tokens per CTA; for up to 32 tokens the weight is the M side of the UMMA,
 //     so that a few tokens cost no padding to 128 rows. K is split over the CTAs of a cluster, which add their partial sums through
-//     distributed shared memory in a fixed order.
-//   * pair_kernel: 256 tokens x 256 outputs per CTA pair, persistent.
+//     distributed shared memory in a fixed order. Bound by the weight's way from HBM and, at these sizes, by what a launch, the first
+//     loads and the exchange take: 1 x 12288 x 4096 13.5 us (50 MB, 3.7 TB/s), 512 x 4096 x 4096 15.8.
+//   * pair_kernel: 256 tokens x 256 outputs per CTA pair, persistent. 8192 x 12288 x 4096 401 to 421 us as the power cap allows
+//     (2.0 PFLOP/s), 4096 x 4096 x 4096 76 to 82.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -120,7 +122,7 @@ __device__ __forceinline__ void let_copies_land(const WaitGuard& guard) {
 // Scales. A load into a register that is used some k blocks later does not work: the loads of all the k blocks in between
 // share the warp's few scoreboards, so the first use waits for the newest of them (3 loads per k block, fetched four ahead,
 // cost the pair kernel 200 of 620 us at 8192 x 12288 x 4096). So one warp brings the scales of k block after k block into
-// shared memory with asynchronous copies, kAhead blocks early, and writes the products sa * sw for the epilogue warps. Its
+// shared memory with asynchronous copies, kScaleAhead blocks early, and writes the products sa * sw for the epilogue warps. Its
 // arrival is the second one on the accumulator's "full" barrier, so the epilogue waits for both at once.
 constexpr int kScaleAhead = 6;
 constexpr int kScaleRing = 8;   // raw scales: more than kScaleAhead, a lane may still read the one before
@@ -515,7 +517,11 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
 // What bounds it is the way of an accumulator from the tensor core through the epilogue's registers and back to the tensor
 // core once per 128-deep block. So a k block's product is two UMMA groups of half the tile's outputs (h = 0, 1: rows
 // h * seg .. of both CTAs' weight boxes), each with two accumulators, barriers and four epilogue warps of its own: the warps of one
-// half load accumulators from tensor memory while those of the other scale theirs.
+// half load accumulators from tensor memory while those of the other scale theirs. A k block takes some 965 clocks of which the
+// tensor core works 512 (52 % of the active cycles at 4096 x 4096 x 4096): from the UMMAs of a half to their commit seen 600 to 770
+// behind those of the other half, loaded, scaled and released 640 to 710, seen by the issuer 250 to 330 later, for two accumulators
+// in turn. Finer groups do not help: four of 64 outputs, released at half the time, take 5 % longer (4096 x 4096 x 4096 85.3 against
+// 81.1 us, twice the barriers), 16 epilogue warps 18 % (90.3 against 76.4: half the registers, so loads and products take turns).
 constexpr int kPairStages = 4;
 constexpr int kPairN = 256;
 constexpr int kPairEpilogueWarps = 8;                              // [half][lane quarter]
@@ -611,8 +617,8 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             }
         } else if ((warp == 1 || warp == 2) && cta == 0 && elect_one()) {
             // ------------------------------------------------------------------ UMMA issuers of the pair, one per half of the outputs. A wait,
-            // even on a barrier that is there, takes the issuing thread 75 clocks and a group with its commits 200: one thread for both
-            // halves was the slowest part of the loop (646 clocks a k block, 512 of the tensor core).
+            // even on a barrier that is there, takes the issuing thread 75 clocks and a group with its commits 200. (One thread for both
+            // halves, which then wait for one another: 4096 x 4096 x 4096 83.7 us, 81.7 with two.)
             const int h = warp - 1;
             Ring slot, out;
             bool ok = true;
