@@ -12,7 +12,7 @@
 //   * small_kernel: 128 outputs x 16, 32 or 128 tokens per CTA; for up to 32 tokens the weight is the M side of the UMMA,
 //     so that a few tokens cost no padding to 128 rows. K is split over the CTAs of a cluster, which add their partial sums through
 //     distributed shared memory in a fixed order. Bound by the weight's way from HBM and, at these sizes, by what a launch, the first
-//     loads and the exchange take: 1 x 12288 x 4096 13.5 us (50 MB, 3.7 TB/s), 512 x 4096 x 4096 15.8.
+//     loads and the exchange take: 1 x 12288 x 4096 12.7 us (50 MB, 4.0 TB/s), 512 x 4096 x 4096 15.8.
 //   * pair_kernel: 256 tokens x 256 outputs per CTA pair, persistent. 8192 x 12288 x 4096 401 to 421 us as the power cap allows
 //     (2.0 PFLOP/s), 4096 x 4096 x 4096 76 to 82.
 #include <cuda_runtime.h>
@@ -188,6 +188,10 @@ __device__ __forceinline__ void quantize_passes(const uint4 (&in)[kQuantizePasse
 // and a column's scale comes from shared memory. With T = 128 the tokens are the M side, so that a lane has one scale per
 // k block and the registers of a warp are outputs. (64 tokens as columns were never faster than 128 lanes: 64 x 5120 x 5120
 // in three K splits 13.0 us against 10.9.)
+// Loads, UMMAs and accumulators are handed over in steps: two k blocks each up to 32 tokens, where a hand-over costs as much as the
+// block's UMMAs (1 x 12288 x 4096 12.7 us, 13.4 with one; 24 x 12288 x 4096 backward without a K split 23.0 and 24.7), one with 128 tokens (128 x 4096 x 4096
+// 11.0, 11.4 with two; 463 x 9600 x 544 18.8 and 19.4). What is left at 16 x 12288 x 4096: 12.6 us, of which HBM needs 7.8 for the
+// weight and the launch, the first loads and the drain some 3.5 (9.6 us with the weight in L2). Tiles of fewer outputs on more SMs take as long.
 template <int T, bool kQuantize>
 struct SmallShape {
     static constexpr bool kTokenLanes = T == 128;
@@ -198,17 +202,21 @@ struct SmallShape {
     static constexpr int kWarps = 4 * kGroups * kTeams;
     static constexpr int kScaleWarps = kQuantize ? kQuantizeWarps : 1;
     static constexpr int kThreads = 32 * (kWarps + 2 + kScaleWarps);     // the last ones load, multiply, and bring the scales or quantize
-    static constexpr int kStageBytes = kTileBytes + T * 128;
-    static constexpr int kStages = T == 16 ? 11 : T == 32 ? 10 : 6;
-    static constexpr int kSlots = T == 128 ? 4 : 8;                      // accumulators in tensor memory
-    static constexpr int kTmemColumns = kSlots * kWidth;
+    static constexpr int kDeep = kTokenLanes ? 1 : 2;                    // k blocks per step
+    static constexpr int kStageBytes = kDeep * (kTileBytes + T * 128);   // weight tiles, then activation tiles
+    static constexpr int kActivationOff = kDeep * kTileBytes;
+    static constexpr int kStages = T == 32 ? 5 : 6;
+    static constexpr int kSlots = 4;                                     // steps whose accumulators are in tensor memory
+    static constexpr int kSlotColumns = kDeep * kWidth;
+    static constexpr int kTmemColumns = kSlots * kSlotColumns;
     static constexpr int kPitch = kTokenLanes ? 132 : 128;               // floats of a token's partial sums (lanes are tokens: no bank twice)
     static constexpr int kRaw = T + 4;                                   // floats: T token scales, the weight's, padding
     static constexpr int kRawOff = kStages * kStageBytes;
-    static constexpr int kBatch = kSlots / 2;                            // k blocks that the scale warp does at a time
-    static constexpr int kRawRing = 4 * kBatch;                          // fetched two batches ahead
-    static constexpr int kScaleOff = kRawOff + kRawRing * kRaw * 4;      // [2 kSlots][T] products
-    static constexpr int kBarOff = kScaleOff + 2 * kSlots * T * 4;
+    static constexpr int kBatch = kSlots / 2;                            // steps that the scale warp does at a time
+    static constexpr int kRawRing = 4 * kBatch * kDeep;                  // k blocks, fetched two batches ahead
+    static constexpr int kProducts = 2 * kSlots * kDeep;                 // k blocks whose products are kept
+    static constexpr int kScaleOff = kRawOff + kRawRing * kRaw * 4;      // [kProducts][T]
+    static constexpr int kBarOff = kScaleOff + kProducts * T * 4;
     static constexpr int kNumBars = 2 * kStages + 2 * kSlots;
     static constexpr int kTotal = kBarOff + kNumBars * 8 + 16;
     static constexpr int kDynamic = kTotal + 1024;
@@ -237,11 +245,11 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
     if (threadIdx.x == 0) {
         *abort_flag = 0u;
         for (int s = 0; s < L::kStages; ++s) {
-            mbar_init(&full[s], kQuantize ? 2 : 1);
+            mbar_init(&full[s], kQuantize ? 1 + L::kDeep : 1);
             mbar_init(&empty[s], 1);
         }
         for (int s = 0; s < L::kSlots; ++s) {
-            mbar_init(&tmem_full[s], 2);
+            mbar_init(&tmem_full[s], kQuantize ? 1 + L::kDeep : 2);
             mbar_init(&tmem_empty[s], 4 * L::kGroups);
         }
         mbar_init_fence();
@@ -270,24 +278,37 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
     const int live = p.M - m0 < T ? p.M - m0 : T;
     const int kb_begin = static_cast<int>(static_cast<int64_t>(p.num_kb) * rank / splits);
     const int blocks = static_cast<int>(static_cast<int64_t>(p.num_kb) * (rank + 1) / splits) - kb_begin;
+    constexpr int kDeep = L::kDeep;
+    const int steps = (blocks + kDeep - 1) / kDeep;   // the last one may have fewer k blocks
 
     if (warp == L::kWarps) {
         // ---------------------------------------------------------------------- loads
         if (elect_one()) {
             const auto load_weight = [&](int i, int slot) {
-                const int depth0 = (kb_begin + i) * kBlock;
-                mbar_arrive_expect_tx(&full[slot], kQuantize ? kTileBytes : L::kStageBytes);
-                tma_load_2d(smem + slot * L::kStageBytes, &map_w, &full[slot], kBackward ? n0 : depth0, kBackward ? depth0 : n0);
+                const int here = blocks - i * kDeep < kDeep ? blocks - i * kDeep : kDeep;
+                uint8_t* const stage = smem + slot * L::kStageBytes;
+                mbar_arrive_expect_tx(&full[slot], here * (kTileBytes + (kQuantize ? 0 : T * kBlock)));
+#pragma unroll
+                for (int d = 0; d < kDeep; ++d) {
+                    const int depth0 = (kb_begin + i * kDeep + d) * kBlock;
+                    if (d < here) tma_load_2d(stage + d * kTileBytes, &map_w, &full[slot], kBackward ? n0 : depth0, kBackward ? depth0 : n0);
+                }
             };
             // behind the quantizer the weight fills the ring while that runs
-            const int early = p.weight_ready ? (blocks < L::kStages ? blocks : L::kStages) : 0;
+            const int early = p.weight_ready ? (steps < L::kStages ? steps : L::kStages) : 0;
             for (int i = 0; i < early; ++i) load_weight(i, i);
             grid_dependency_wait();
             Ring slot;
-            for (int i = 0; i < blocks; ++i) {
+            for (int i = 0; i < steps; ++i) {
                 if (!guard.wait(&empty[slot.idx], slot.phase ^ 1u, kSiteLoadEmpty)) break;
                 if (i >= early) load_weight(i, static_cast<int>(slot.idx));
-                if constexpr (!kQuantize) tma_load_2d(smem + slot.idx * L::kStageBytes + kTileBytes, &map_a, &full[slot.idx], (kb_begin + i) * kBlock, m0);
+                if constexpr (!kQuantize) {
+#pragma unroll
+                    for (int d = 0; d < kDeep; ++d) {
+                        const int at = i * kDeep + d;
+                        if (at < blocks) tma_load_2d(smem + slot.idx * L::kStageBytes + L::kActivationOff + d * T * kBlock, &map_a, &full[slot.idx], (kb_begin + at) * kBlock, m0);
+                    }
+                }
                 slot.advance(L::kStages);
             }
         }
@@ -295,17 +316,22 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
         // ---------------------------------------------------------------------- multiplies
         if (elect_one()) {
             Ring slot, out;
-            for (int i = 0; i < blocks; ++i) {
+            for (int i = 0; i < steps; ++i) {
                 if (!guard.wait(&tmem_empty[out.idx], out.phase ^ 1u, kSiteTmemEmpty)) break;
                 if (!guard.wait(&full[slot.idx], slot.phase, kSiteLoadFull)) break;
                 tc_fence_after_sync();
-                const uint32_t w_addr = smem_u32(smem + slot.idx * L::kStageBytes);
-                const uint32_t a_addr = w_addr + kTileBytes;
+                const uint32_t stage = smem_u32(smem + slot.idx * L::kStageBytes);
 #pragma unroll
-                for (int k = 0; k < kBlock / 32; ++k) {
-                    const uint64_t desc_w = kBackward ? make_desc_sw128_mnmajor(w_addr + k * 32 * 128) : make_desc_sw128_kmajor(w_addr + k * 32);
-                    const uint64_t desc_a = make_desc_sw128_kmajor(a_addr + k * 32);
-                    umma_f8(tmem_base + out.idx * L::kWidth, L::kTokenLanes ? desc_a : desc_w, L::kTokenLanes ? desc_w : desc_a, p.idesc, k != 0 ? 1u : 0u);
+                for (int d = 0; d < kDeep; ++d) {
+                    if (i * kDeep + d >= blocks) break;
+                    const uint32_t w_addr = stage + d * kTileBytes;
+                    const uint32_t a_addr = stage + L::kActivationOff + d * T * kBlock;
+#pragma unroll
+                    for (int k = 0; k < kBlock / 32; ++k) {
+                        const uint64_t desc_w = kBackward ? make_desc_sw128_mnmajor(w_addr + k * 32 * 128) : make_desc_sw128_kmajor(w_addr + k * 32);
+                        const uint64_t desc_a = make_desc_sw128_kmajor(a_addr + k * 32);
+                        umma_f8(tmem_base + out.idx * L::kSlotColumns + d * L::kWidth, L::kTokenLanes ? desc_a : desc_w, L::kTokenLanes ? desc_w : desc_a, p.idesc, k != 0 ? 1u : 0u);
+                    }
                 }
                 umma_commit(&empty[slot.idx]);
                 umma_commit(&tmem_full[out.idx]);
@@ -334,20 +360,21 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
         };
         // the ring's rows past the last token are zero, once and for all
         const int spare = (T - live) * 8;
-        for (int i = first * 32 + lane; i < spare * L::kStages; i += 32 * L::kScaleWarps) {
-            *reinterpret_cast<uint4*>(smem + i / spare * L::kStageBytes + kTileBytes + live * 128 + i % spare * 16) = make_uint4(0, 0, 0, 0);
+        for (int i = first * 32 + lane; i < spare * L::kStages * kDeep; i += 32 * L::kScaleWarps) {
+            const int tile_at = i / spare;
+            *reinterpret_cast<uint4*>(smem + tile_at / kDeep * L::kStageBytes + L::kActivationOff + (tile_at % kDeep * T + live) * kBlock + i % spare * 16) = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
         asm volatile("bar.sync 1, %0;" ::"n"(32 * L::kScaleWarps) : "memory");
         grid_dependency_wait();
         fetch(first);
-        for (int i = first; i < blocks; i += L::kScaleWarps) {
-            const int slot = i % L::kStages, at = i % L::kSlots, before = i - L::kSlots;
-            if (!warp_wait(guard, &empty[slot], (static_cast<uint32_t>(i / L::kStages) & 1u) ^ 1u, kSiteOperandEmpty)) break;
-            // the accumulator's previous product is complete, as for the scale warp below
+        for (int i = first; i < steps * kDeep; i += L::kScaleWarps) {   // past the last block: arrivals only
+            const int at = i / kDeep, slot = at % L::kStages, before = at - L::kSlots;
+            if (!warp_wait(guard, &empty[slot], (static_cast<uint32_t>(at / L::kStages) & 1u) ^ 1u, kSiteOperandEmpty)) break;
+            // the slot's previous products are complete, as for the scale warp below
             if (before >= 0 && !warp_wait(guard, &tmem_full[before % L::kSlots], static_cast<uint32_t>(before / L::kSlots) & 1u, kSiteTmemFull)) break;
-            uint8_t* const rows = smem + slot * L::kStageBytes + kTileBytes;
-            float* const product = products + i % (2 * L::kSlots) * T;
+            uint8_t* const rows = smem + slot * L::kStageBytes + L::kActivationOff + i % kDeep * T * kBlock;
+            float* const product = products + i % L::kProducts * T;
             if (p.x_fp16) {
                 p.x_e5m2 ? quantize_passes<true, true>(in, live, sw, rows, product) : quantize_passes<true, false>(in, live, sw, rows, product);
             } else {
@@ -357,20 +384,20 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(&full[slot]);
-                mbar_arrive(&tmem_full[at]);
+                mbar_arrive(&tmem_full[at % L::kSlots]);
             }
             fetch(i + L::kScaleWarps);
         }
     } else if (warp == L::kWarps + 2) {
         // ---------------------------------------------------------------------- scales, kBatch k blocks at a time
-        constexpr int kBatch = L::kBatch;
+        constexpr int kBatch = L::kBatch, kFetch = kBatch * kDeep;   // steps, k blocks
         float* const raw = reinterpret_cast<float*>(smem + L::kRawOff);
         float* const products = reinterpret_cast<float*>(smem + L::kScaleOff);
         const float* a_scale = p.a_scale + static_cast<int64_t>(kb_begin) * p.M + m0;
         const float* w_scale = p.w_scale + tile_n * p.w_scale_out + kb_begin * p.w_scale_block;
         const auto fetch = [&](int i0) {
 #pragma unroll
-            for (int j = 0; j < kBatch; ++j) {
+            for (int j = 0; j < kFetch; ++j) {
                 if (i0 + j < blocks) {
                     fetch_scales<T>(raw + (i0 + j) % L::kRawRing * L::kRaw, a_scale, live, w_scale, w_scale);
                     a_scale += p.M;
@@ -381,24 +408,25 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
         };
         grid_dependency_wait();
         fetch(0);
-        fetch(kBatch);
-        for (int i0 = 0; i0 < blocks; i0 += kBatch) {
+        fetch(kFetch);
+        for (int i0 = 0; i0 < steps; i0 += kBatch) {
             cp_async_wait<1>();
             __syncwarp();
-            // The accumulators' previous products are complete (they come in order, so the last one's is enough): these arrivals
-            // count for the next ones, and the scales of two products ago, which stood where these go, have been read.
+            // The slots' previous products are complete (they come in order, so the last one's is enough): these arrivals
+            // count for the next ones, and the scales of two turns ago, which stood where these go, have been read.
             const int before = i0 + kBatch - 1 - L::kSlots;
             if (before >= 0 && !warp_wait(guard, &tmem_full[before % L::kSlots], static_cast<uint32_t>(before / L::kSlots) & 1u, kSiteTmemFull)) break;
 #pragma unroll
-            for (int j = 0; j < kBatch; ++j) {
-                const float* const from = raw + (i0 + j) % L::kRawRing * L::kRaw;
+            for (int j = 0; j < kFetch; ++j) {
+                const int at = i0 * kDeep + j;
+                const float* const from = raw + at % L::kRawRing * L::kRaw;
                 const float w = from[T];   // of blocks past the end: whatever stands there, nobody reads the products
 #pragma unroll
-                for (int r = lane; r < T; r += 32) products[(i0 + j) % (2 * L::kSlots) * T + r] = from[r] * w;
+                for (int r = lane; r < T; r += 32) products[at % L::kProducts * T + r] = from[r] * w;
             }
-            fetch(i0 + 2 * kBatch);
+            fetch(i0 * kDeep + 2 * kFetch);
             __syncwarp();
-            if (lane < kBatch && i0 + lane < blocks) mbar_arrive(&tmem_full[(i0 + lane) % L::kSlots]);
+            if (lane < kBatch && i0 + lane < steps) mbar_arrive(&tmem_full[(i0 + lane) % L::kSlots]);
         }
         cp_async_wait<0>();
     } else {
@@ -415,32 +443,41 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
         for (int t = 0; t < kColumns / 2; ++t) acc[t] = make_float2(0.0f, 0.0f);
         bool ok = true;
 #pragma unroll 1
-        for (int i = team; i < blocks; i += L::kTeams) {
+        for (int i = team; i < steps; i += L::kTeams) {
             const int at = i % L::kSlots;
             ok = warp_wait(guard, &tmem_full[at], static_cast<uint32_t>(i / L::kSlots) & 1u, kSiteTmemFull);
             if (!ok) break;
             tc_fence_after_sync();
-            const float* const scales = products + i % (2 * L::kSlots) * T;
+            const float* const scales = products + i * kDeep % L::kProducts * T;
+            const uint32_t from = taddr + at * L::kSlotColumns;
             if constexpr (L::kTokenLanes) {
-                uint32_t v[2][32];
                 static_assert(kColumns == 64, "two loads of 32 columns");
-                tmem_ld_32x32(taddr + at * L::kWidth, v[0]);
-                tmem_ld_32x32(taddr + at * L::kWidth + 32, v[1]);
-                const float s = scales[token];
-                tmem_wait_ld();
 #pragma unroll
-                for (int g = 0; g < 64; g += 2) fma2(acc[g / 2], v[g / 32][g % 32], v[g / 32][g % 32 + 1], s, s);
-            } else {
-#pragma unroll
-                for (int c = 0; c < kColumns; c += 16) {
-                    uint32_t v[16];
-                    tmem_ld_32x16(taddr + at * L::kWidth + c, v);
+                for (int d = 0; d < kDeep; ++d) {
+                    if (i * kDeep + d >= blocks) break;
+                    uint32_t v[2][32];
+                    tmem_ld_32x32(from + d * L::kWidth, v[0]);
+                    tmem_ld_32x32(from + d * L::kWidth + 32, v[1]);
+                    const float s = scales[d * T + token];
                     tmem_wait_ld();
 #pragma unroll
-                    for (int g = 0; g < 16; g += 4) {
-                        const float4 f = *reinterpret_cast<const float4*>(scales + column0 + c + g);
-                        fma2(acc[(c + g) / 2], v[g], v[g + 1], f.x, f.y);
-                        fma2(acc[(c + g) / 2 + 1], v[g + 2], v[g + 3], f.z, f.w);
+                    for (int g = 0; g < 64; g += 2) fma2(acc[g / 2], v[g / 32][g % 32], v[g / 32][g % 32 + 1], s, s);
+                }
+            } else {
+                // All of the step's loads before the first product. Past the last block stands whatever was there: not used.
+                uint32_t v[kDeep * T / 16][16];
+#pragma unroll
+                for (int c = 0; c < kDeep * T / 16; ++c) tmem_ld_32x16(from + c * 16, v[c]);
+                tmem_wait_ld();
+#pragma unroll
+                for (int d = 0; d < kDeep; ++d) {
+                    if (i * kDeep + d >= blocks) break;
+#pragma unroll
+                    for (int t = 0; t < T; t += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(scales + d * T + t);
+                        const uint32_t* const c = v[(d * T + t) / 16] + t % 16;
+                        fma2(acc[t / 2], c[0], c[1], f.x, f.y);
+                        fma2(acc[t / 2 + 1], c[2], c[3], f.z, f.w);
                     }
                 }
             }
@@ -450,8 +487,8 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
         }
         // Every team's sums go into this CTA's operand ring, [team][token][output]. A team may be ahead of the last block's
         // UMMAs, which still read the ring.
-        if (ok && blocks > 0) {
-            const int last = blocks - 1;
+        if (ok && steps > 0) {
+            const int last = steps - 1;
             (void)warp_wait(guard, &tmem_full[last % L::kSlots], static_cast<uint32_t>(last / L::kSlots) & 1u, kSiteTmemFull);
         }
         float* const part = reinterpret_cast<float*>(smem) + team * T * L::kPitch;
