@@ -11,20 +11,19 @@ import sys
 
 import torch  # noqa: F401  the extension links against libtorch, so torch has to be loaded first
 
-# `python -m feather_ops_b200._build` imports this package before it runs the build script: that one entry has to get
-# through without the extension, everything else fails loudly.
+# `python -m feather_ops_b200._build` imports this package before it runs the build script: that one entry gets through without
+# the extension (an older one may lack operators that the modules below register for), everything else fails loudly.
 _BUILDING = "feather_ops_b200._build" in getattr(sys, "orig_argv", [])
 
-try:
-    from . import _C  # noqa: F401  registers torch.ops.feather_ops.{scaled_mm,int8_scaled_mm,convrot_quantize,conv2d_3x3,...}
-except ImportError as exc:  # pragma: no cover - depends on the build state
-    if not _BUILDING:
+if not _BUILDING:
+    try:
+        from . import _C  # noqa: F401  registers torch.ops.feather_ops.{scaled_mm,int8_scaled_mm,convrot_quantize,conv2d_3x3,...}
+    except ImportError as exc:  # pragma: no cover - depends on the build state
         raise ImportError(
             "feather_ops_b200._C is not built (or failed to load): run `python -m feather_ops_b200._build` "
             "(needs nvcc and g++, no GPU). The kernels have no fallback path."
         ) from exc
 
-if not _BUILDING or "feather_ops_b200._C" in sys.modules:
     from .conv2d import conv3x3_prepacked, prepack_conv2d_weight_3x3
     from .conv2d_module import Conv2d
     from .fp8_block import (

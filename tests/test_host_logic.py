@@ -172,3 +172,16 @@ def test_public_api_surface():
     with pytest.raises((RuntimeError, NotImplementedError)):
         torch.ops.feather_ops.scaled_mm.default(x, torch.zeros(8, 16, 16).to(torch.float8_e5m2), None, None, torch.zeros(4, 16, dtype=torch.float16), 1, 8, 4, 8, 2, False)
     assert oc.prepack_conv2d_weight_3x3(torch.zeros(4, 8, 3, 3)).shape == (18, 4, 8)
+
+
+def test_build_entry_loads_no_extension():
+    """`python -m feather_ops_b200._build` has to work beside an extension of an older source tree: the package it imports first must
+    not load one."""
+    import subprocess
+    import sys
+
+    code = (
+        "import sys; sys.orig_argv = [sys.executable, '-m', 'feather_ops_b200._build']; import feather_ops_b200; "
+        "sys.exit('feather_ops_b200._C' in sys.modules)"
+    )
+    assert subprocess.run([sys.executable, "-c", code], cwd=_build.ROOT).returncode == 0
