@@ -453,28 +453,35 @@ void check_norm_weight(const Tensor& weight, const Tensor& x, int64_t K) {
     STD_TORCH_CHECK(K <= 32768, "a norm's rows may have at most 32768 channels");
 }
 
-std::tuple<Tensor, Tensor, Tensor> rms_norm_fp8(const Tensor& x, const std::optional<Tensor>& residual, const Tensor& weight,
-                                                std::optional<Tensor> residual_out, double eps, bool e5m2) {
+// `stream`: receives x + residual (both null without a residual).
+std::tuple<Tensor, Tensor, Tensor> norm_codes(const Tensor& x, const Tensor* residual, const Tensor& weight, double eps, bool e5m2, Tensor* stream) {
     check_input(x, "x", 16);
     const auto device = x.get_device_index();
     const int64_t M = x.size(0), K = x.size(1);
-    STD_TORCH_CHECK(residual.has_value() == residual_out.has_value(), "residual and residual_out come together");
-    if (residual.has_value()) {
-        check_rows(*residual, "residual", M, K, x.scalar_type(), device);
-        check_rows(*residual_out, "residual_out", M, K, x.scalar_type(), device);
-    }
+    if (residual != nullptr) check_rows(*residual, "residual", M, K, x.scalar_type(), device);
     check_norm_weight(weight, x, K);
     STD_TORCH_CHECK(eps >= 0, "eps must not be negative");
     torch::stable::accelerator::DeviceGuard guard(device);
+    if (stream != nullptr) *stream = make_empty({M, K}, half_dtype(is_half(x)), device);
     Tensor q = make_empty({M, K}, code_dtype(e5m2), device);
     Tensor scale = make_empty({blocks_of(K), M}, aoti_torch_dtype_float32(), device);
     Tensor rstd = make_empty({M}, aoti_torch_dtype_float32(), device);
-    const bool ok = launch_rms_norm_fp8(x.const_data_ptr(), residual.has_value() ? residual->const_data_ptr() : nullptr, weight.const_data_ptr(),
-                                        residual_out.has_value() ? residual_out->mutable_data_ptr() : nullptr, q.mutable_data_ptr(),
+    const bool ok = launch_rms_norm_fp8(x.const_data_ptr(), residual != nullptr ? residual->const_data_ptr() : nullptr, weight.const_data_ptr(),
+                                        stream != nullptr ? stream->mutable_data_ptr() : nullptr, q.mutable_data_ptr(),
                                         static_cast<float*>(scale.mutable_data_ptr()), static_cast<float*>(rstd.mutable_data_ptr()), M, K, static_cast<float>(eps),
                                         is_half(x) ? 1 : 0, weight.scalar_type() == ScalarType::Float ? 1 : 0, e5m2 ? 1 : 0, current_stream(device));
     STD_TORCH_CHECK(ok, "rms_norm_fp8 launch failed");
     return std::make_tuple(std::move(q), std::move(scale), std::move(rstd));
+}
+
+std::tuple<Tensor, Tensor, Tensor> rms_norm_fp8(const Tensor& x, const Tensor& weight, double eps, bool e5m2) {
+    return norm_codes(x, nullptr, weight, eps, e5m2, nullptr);
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> add_rms_norm_fp8(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps, bool e5m2) {
+    Tensor stream;
+    auto [q, scale, rstd] = norm_codes(x, &residual, weight, eps, e5m2, &stream);
+    return std::make_tuple(std::move(q), std::move(scale), std::move(rstd), std::move(stream));
 }
 
 std::tuple<Tensor, Tensor> rms_norm_dgrad(const Tensor& grad, const Tensor& x, const Tensor& weight, const Tensor& rstd,
@@ -606,8 +613,8 @@ STABLE_TORCH_LIBRARY(feather_ops, m) {
     m.def(
         "fp8_block_mm(Tensor a, Tensor a_scale, Tensor weight, Tensor weight_scale, Tensor? bias, bool out_fp16, bool transposed_b) -> Tensor");
     m.def("fp8_block_linear(Tensor x, Tensor weight, Tensor weight_scale, Tensor? bias, bool out_fp16, bool transposed_b, bool e5m2) -> Tensor");
-    m.def(
-        "rms_norm_fp8(Tensor x, Tensor? residual, Tensor weight, Tensor(a!)? residual_out, float eps, bool e5m2) -> (Tensor, Tensor, Tensor)");
+    m.def("rms_norm_fp8(Tensor x, Tensor weight, float eps, bool e5m2) -> (Tensor, Tensor, Tensor)");
+    m.def("add_rms_norm_fp8(Tensor x, Tensor residual, Tensor weight, float eps, bool e5m2) -> (Tensor, Tensor, Tensor, Tensor)");
     m.def("rms_norm_dgrad(Tensor grad, Tensor x, Tensor weight, Tensor rstd, Tensor? grad_residual) -> (Tensor, Tensor)");
     m.def("silu_mul_fp8(Tensor gate_up, bool e5m2) -> (Tensor, Tensor)");
     m.def("silu_mul_dgrad(Tensor grad, Tensor gate_up) -> Tensor");
@@ -627,6 +634,7 @@ STABLE_TORCH_LIBRARY_IMPL(feather_ops, CUDA, m) {
     m.impl("fp8_block_mm", TORCH_BOX(&fp8_block_mm));
     m.impl("fp8_block_linear", TORCH_BOX(&fp8_block_linear));
     m.impl("rms_norm_fp8", TORCH_BOX(&rms_norm_fp8));
+    m.impl("add_rms_norm_fp8", TORCH_BOX(&add_rms_norm_fp8));
     m.impl("rms_norm_dgrad", TORCH_BOX(&rms_norm_dgrad));
     m.impl("silu_mul_fp8", TORCH_BOX(&silu_mul_fp8));
     m.impl("silu_mul_dgrad", TORCH_BOX(&silu_mul_dgrad));

@@ -130,10 +130,9 @@ def rms_norm_quantize_fp8(x, weight, residual=None, eps=1e-6, dtype=torch.float8
         raise ValueError(f"residual is {tuple(residual.shape)}, x {tuple(x.shape)}")
     rows = _rows(x)
     if residual is None:
-        q, scale, rstd = _ops.rms_norm_fp8.default(rows, None, weight, None, eps, _is_e5m2(dtype))
+        q, scale, rstd = _ops.rms_norm_fp8.default(rows, weight, eps, _is_e5m2(dtype))
         return q, scale, x, rstd
-    stream = torch.empty_like(rows)
-    q, scale, rstd = _ops.rms_norm_fp8.default(rows, _rows(residual), weight, stream, eps, _is_e5m2(dtype))
+    q, scale, rstd, stream = _ops.add_rms_norm_fp8.default(rows, _rows(residual), weight, eps, _is_e5m2(dtype))
     return q, scale, stream.view(x.shape) if x.ndim != 2 else stream, rstd
 
 
@@ -190,8 +189,13 @@ def _(x, weight, weight_scale, bias, out_fp16, transposed_b, e5m2):
 
 
 @torch.library.register_fake("feather_ops::rms_norm_fp8")
-def _(x, residual, weight, residual_out, eps, e5m2):
+def _(x, weight, eps, e5m2):
     return *_fake_codes(x.shape[0], x.shape[1], x, e5m2), x.new_empty((x.shape[0],), dtype=torch.float32)
+
+
+@torch.library.register_fake("feather_ops::add_rms_norm_fp8")
+def _(x, residual, weight, eps, e5m2):
+    return *_fake_codes(x.shape[0], x.shape[1], x, e5m2), x.new_empty((x.shape[0],), dtype=torch.float32), torch.empty_like(x)
 
 
 @torch.library.register_fake("feather_ops::rms_norm_dgrad")
