@@ -1075,20 +1075,23 @@ double pair_cost(const Args& args) {
     return 4.2 + static_cast<double>((tiles + pairs - 1) / pairs) * (1.3 + 0.46 * static_cast<double>(num_kb));
 }
 
-// Up to 16 tokens one tile of 16. Above, the cheapest of tiles of 32 (up to 128 tokens), tiles of 128 and the pair kernel. Measured (us): 78 x 6016 x
-// 640 5.2 with tiles of 32 and 6.0 of 128, 64 x 5120 x 5120 13.5 and 10.9; 512 x 4096 x 4096 15.8 with tiles of 128 and 21.1 on the pair kernel,
-// 744 x 7872 x 560 22.0 and 12.6, 1024 x 4096 x 4096 33.7 and 22.2.
+// Up to 16 tokens one tile of 16. Above, the cheapest of tiles of 16 (up to 64 tokens), of 32 (up to 128), of 128 and the pair kernel. Measured
+// (us): 47 x 608 x 3888 backward 5.3 with tiles of 16 and 5.8 of 32, 26 x 10880 x 1568 13.3 and 7.8; 78 x 6016 x 640 5.2 with tiles of 32 and 6.0 of
+// 128, 64 x 5120 x 5120 13.5 and 10.9; 512 x 4096 x 4096 15.8 with tiles of 128 and 21.1 on the pair kernel, 744 x 7872 x 560 22.0 and 12.6, 1024 x 4096 x
+// 4096 33.7 and 22.2.
 template <bool kBackward, bool kOutBf16>
 bool launch(const Args& args) {
     if (args.x != nullptr) return launch_small<16, kBackward, kOutBf16, true>(args, small_choice<16, kBackward, kOutBf16, true>(args).splits);
     if (args.M <= 16) return launch_small<16, kBackward, kOutBf16, false>(args, small_choice<16, kBackward, kOutBf16, false>(args).splits);
-    Choice narrow{1e30, 1}, wide{1e30, 1};
+    Choice least{1e30, 1}, narrow{1e30, 1}, wide{1e30, 1};
     double pair = 1e30;
+    if (args.M <= 64) least = small_choice<16, kBackward, kOutBf16, false>(args);
     if (args.M <= 128) narrow = small_choice<32, kBackward, kOutBf16, false>(args);
     if (args.M > 32) {
         wide = small_choice<128, kBackward, kOutBf16, false>(args);
         pair = pair_cost(args);
     }
+    if (least.cost < narrow.cost && least.cost < wide.cost && least.cost < pair) return launch_small<16, kBackward, kOutBf16, false>(args, least.splits);
     if (narrow.cost <= wide.cost && narrow.cost <= pair) return launch_small<32, kBackward, kOutBf16, false>(args, narrow.splits);
     if (wide.cost <= pair) return launch_small<128, kBackward, kOutBf16, false>(args, wide.splits);
     return launch_pair<kBackward, kOutBf16>(args);

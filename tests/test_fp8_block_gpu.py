@@ -106,6 +106,28 @@ def test_product(cuda_device, shape, transposed):
     _product_close(out, q, s, w, ws, None, transposed)
 
 
+# Many outputs and 17 to 128 tokens: tiles of 32 tokens, one K split, odd and even numbers of k blocks.
+@pytest.mark.parametrize("transposed", [False, True], ids=["forward", "backward"])
+@pytest.mark.parametrize("shape", [(18, 10880, 128), (26, 10880, 400), (31, 9600, 272), (54, 7872, 560), (90, 6016, 656), (128, 4112, 144)], ids=lambda s: "x".join(map(str, s)))
+def test_product_with_many_outputs(cuda_device, shape, transposed):
+    m, n, k = shape if not transposed else (shape[0], shape[2], shape[1])
+    q, s, w, ws = _operands(m, n, k, E4M3, E5M2, transposed, seed=sum(shape))
+    out = fo.fp8_block_mm(q, s, w, ws, None, torch.bfloat16, transposed)
+    _product_close(out, q, s, w, ws, None, transposed)
+
+
+@pytest.mark.parametrize("m", [1, 20, 45, 300, 900])
+def test_the_same_bits_on_every_run(cuda_device, m):
+    x, w, ws = _rand(m, 2064, torch.bfloat16, 1).cuda(), *(t.cuda() for t in fo.quantize_fp8_weight(_rand(1040, 2064, torch.float32, 2, 0.02)))
+    rstd, nw = torch.ones(m, device=cuda_device), _rand(1, 2064, torch.bfloat16, 3)[0].cuda()
+    first = None
+    for _ in range(4):
+        dx, dw = fo.rms_norm_dgrad(x.flip(1).contiguous(), x, nw, rstd)
+        got = [fo.fp8_block_linear(x, w, ws), fo.fp8_block_dgrad(fo.fp8_block_linear(x, w, ws), w, ws), dx, dw]
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(first, got))
+
+
 @pytest.mark.parametrize("transposed", [False, True], ids=["forward", "backward"])
 @pytest.mark.parametrize("out_type", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("w_type", [E4M3, E5M2])
