@@ -200,7 +200,7 @@ struct SmallShape {
     static constexpr int kGroups = kWidth / kColumns;
     static constexpr int kTeams = kTokenLanes ? 1 : 2;                   // teams take the k blocks in turn
     static constexpr int kWarps = 4 * kGroups * kTeams;
-    static constexpr int kScaleWarps = kQuantize ? kQuantizeWarps : 1;
+    static constexpr int kScaleWarps = kQuantize ? kQuantizeWarps : 2;
     static constexpr int kThreads = 32 * (kWarps + 2 + kScaleWarps);     // the last ones load, multiply, and bring the scales or quantize
     static constexpr int kDeep = kTokenLanes ? 1 : 2;                    // k blocks per step
     static constexpr int kStageBytes = kDeep * (kTileBytes + T * 128);   // weight tiles, then activation tiles
@@ -212,8 +212,8 @@ struct SmallShape {
     static constexpr int kPitch = kTokenLanes ? 132 : 128;               // floats of a token's partial sums (lanes are tokens: no bank twice)
     static constexpr int kRaw = T + 4;                                   // floats: T token scales, the weight's, padding
     static constexpr int kRawOff = kStages * kStageBytes;
-    static constexpr int kBatch = kSlots / 2;                            // steps that the scale warp does at a time
-    static constexpr int kRawRing = 4 * kBatch * kDeep;                  // k blocks, fetched two batches ahead
+    static constexpr int kBatch = kSlots / 2;                            // steps that a scale warp does at a time
+    static constexpr int kRawRing = kQuantize ? 0 : 4 * kScaleWarps * kBatch * kDeep;   // k blocks, a warp's fetched two batches ahead
     static constexpr int kProducts = 2 * kSlots * kDeep;                 // k blocks whose products are kept
     static constexpr int kScaleOff = kRawOff + kRawRing * kRaw * 4;      // [kProducts][T]
     static constexpr int kBarOff = kScaleOff + kProducts * T * 4;
@@ -388,28 +388,30 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
             }
             fetch(i + L::kScaleWarps);
         }
-    } else if (warp == L::kWarps + 2) {
-        // ---------------------------------------------------------------------- scales, kBatch k blocks at a time
+    } else if (warp >= L::kWarps + 2) {
+        // ---------------------------------------------------------------------- scales, kBatch steps at a time, the warps in turn
         constexpr int kBatch = L::kBatch, kFetch = kBatch * kDeep;   // steps, k blocks
+        constexpr int kTurn = L::kScaleWarps * kBatch;
         float* const raw = reinterpret_cast<float*>(smem + L::kRawOff);
         float* const products = reinterpret_cast<float*>(smem + L::kScaleOff);
-        const float* a_scale = p.a_scale + static_cast<int64_t>(kb_begin) * p.M + m0;
-        const float* w_scale = p.w_scale + tile_n * p.w_scale_out + kb_begin * p.w_scale_block;
+        const float* const a_scale = p.a_scale + static_cast<int64_t>(kb_begin) * p.M + m0;
+        const float* const w_scale = p.w_scale + tile_n * p.w_scale_out + kb_begin * p.w_scale_block;
         const auto fetch = [&](int i0) {
 #pragma unroll
             for (int j = 0; j < kFetch; ++j) {
-                if (i0 + j < blocks) {
-                    fetch_scales<T>(raw + (i0 + j) % L::kRawRing * L::kRaw, a_scale, live, w_scale, w_scale);
-                    a_scale += p.M;
-                    w_scale += p.w_scale_block;
+                const int at = i0 * kDeep + j;
+                if (at < blocks) {
+                    const float* const w = w_scale + at * p.w_scale_block;
+                    fetch_scales<T>(raw + at % L::kRawRing * L::kRaw, a_scale + static_cast<int64_t>(at) * p.M, live, w, w);
                 }
             }
             cp_async_commit();
         };
         grid_dependency_wait();
-        fetch(0);
-        fetch(kFetch);
-        for (int i0 = 0; i0 < steps; i0 += kBatch) {
+        const int first = (warp - (L::kWarps + 2)) * kBatch;
+        fetch(first);
+        fetch(first + kTurn);
+        for (int i0 = first; i0 < steps; i0 += kTurn) {
             cp_async_wait<1>();
             __syncwarp();
             // The slots' previous products are complete (they come in order, so the last one's is enough): these arrivals
@@ -421,12 +423,14 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
                 const int at = i0 * kDeep + j;
                 const float* const from = raw + at % L::kRawRing * L::kRaw;
                 const float w = from[T];   // of blocks past the end: whatever stands there, nobody reads the products
-#pragma unroll
-                for (int r = lane; r < T; r += 32) products[at % L::kProducts * T + r] = from[r] * w;
+                if (lane < T / 4) {
+                    const float4 a = reinterpret_cast<const float4*>(from)[lane];
+                    reinterpret_cast<float4*>(products + at % L::kProducts * T)[lane] = make_float4(a.x * w, a.y * w, a.z * w, a.w * w);
+                }
             }
-            fetch(i0 * kDeep + 2 * kFetch);
             __syncwarp();
             if (lane < kBatch && i0 + lane < steps) mbar_arrive(&tmem_full[(i0 + lane) % L::kSlots]);
+            fetch(i0 + 2 * kTurn);
         }
         cp_async_wait<0>();
     } else {
@@ -737,20 +741,14 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     break;
                 }
                 const float* const from = raw + turn % kScaleRing * L::kRaw;
-                float* const to = products + (turn & 3u) * 256;
+                const float4 a = reinterpret_cast<const float4*>(from)[lane];
                 const float s0 = from[128], s1 = from[129];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float sa = from[r * 32 + lane];
-                    to[r * 32 + lane] = sa * s0;
-                    to[128 + r * 32 + lane] = sa * s1;
-                }
-                fetch(turn + kScaleAhead);
+                float4* const to = reinterpret_cast<float4*>(products + (turn & 3u) * 256) + lane;
+                to[0] = make_float4(a.x * s0, a.y * s0, a.z * s0, a.w * s0);
+                to[32] = make_float4(a.x * s1, a.y * s1, a.z * s1, a.w * s1);
                 __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&tmem_full[slot]);
-                    mbar_arrive(&tmem_full[2 + slot]);
-                }
+                if (lane < 2) mbar_arrive(&tmem_full[2 * lane + slot]);
+                fetch(turn + kScaleAhead);
             }
             cp_async_wait<0>();
         }
