@@ -12,9 +12,9 @@
 //   * small_kernel: 128 outputs x 16, 32 or 128 tokens per CTA; for up to 32 tokens the weight is the M side of the UMMA,
 //     so that a few tokens cost no padding to 128 rows. K is split over the CTAs of a cluster, which add their partial sums through
 //     distributed shared memory in a fixed order. Bound by the weight's way from HBM and, at these sizes, by what a launch, the first
-//     loads and the exchange take: 1 x 12288 x 4096 12.7 us (50 MB, 4.0 TB/s), 512 x 4096 x 4096 15.8.
-//   * pair_kernel: 256 tokens x 256 outputs per CTA pair, persistent. 8192 x 12288 x 4096 401 to 421 us as the power cap allows
-//     (2.0 PFLOP/s), 4096 x 4096 x 4096 76 to 82.
+//     loads and the exchange take: 1 x 12288 x 4096 12.7 us (50 MB, 4.0 TB/s), 512 x 4096 x 4096 14.1.
+//   * pair_kernel: 256 tokens x 256 outputs per CTA pair, persistent. 8192 x 12288 x 4096 386 to 405 us as the power cap allows
+//     (2.1 PFLOP/s), 4096 x 4096 x 4096 65.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -121,9 +121,11 @@ __device__ __forceinline__ void let_copies_land(const WaitGuard& guard) {
 
 // Scales. A load into a register that is used some k blocks later does not work: the loads of all the k blocks in between
 // share the warp's few scoreboards, so the first use waits for the newest of them (3 loads per k block, fetched four ahead,
-// cost the pair kernel 200 of 620 us at 8192 x 12288 x 4096). So one warp brings the scales of k block after k block into
-// shared memory with asynchronous copies, kScaleAhead blocks early, and writes the products sa * sw for the epilogue warps. Its
-// arrival is the second one on the accumulator's "full" barrier, so the epilogue waits for both at once.
+// cost the pair kernel 200 of 620 us at 8192 x 12288 x 4096). So a warp (two in the small kernel, a batch each in turn)
+// brings the scales of k block after k block into shared memory with asynchronous copies, some blocks early, and writes the products
+// sa * sw for the epilogue warps. Its arrival is the second one on the accumulator's "full" barrier, so the epilogue waits for both
+// at once. It has to be quick: four-byte accesses, and its own next copies issued before the arrival, set the pace of both
+// kernels (4096 x 4096 x 4096 69.6 us, 64.9 now and 63.2 without scales; 512 x 4096 x 4096 15.3, 14.1 and 13.8).
 constexpr int kScaleAhead = 6;
 constexpr int kScaleRing = 8;   // raw scales: more than kScaleAhead, a lane may still read the one before
 
@@ -189,8 +191,8 @@ __device__ __forceinline__ void quantize_passes(const uint4 (&in)[kQuantizePasse
 // k block and the registers of a warp are outputs. (64 tokens as columns were never faster than 128 lanes: 64 x 5120 x 5120
 // in three K splits 13.0 us against 10.9.)
 // Loads, UMMAs and accumulators are handed over in steps: two k blocks each up to 32 tokens, where a hand-over costs as much as the
-// block's UMMAs (1 x 12288 x 4096 12.7 us, 13.4 with one; 24 x 12288 x 4096 backward without a K split 23.0 and 24.7), one with 128 tokens (128 x 4096 x 4096
-// 11.0, 11.4 with two; 463 x 9600 x 544 18.8 and 19.4). What is left at 16 x 12288 x 4096: 12.6 us, of which HBM needs 7.8 for the
+// block's UMMAs (1 x 12288 x 4096 12.7 us, 13.4 with one; 24 x 12288 x 4096 backward without a K split 23.0 and 24.7 at the time), one with 128 tokens (128 x 4096 x 4096
+// 11.0, 11.4 with two; 888 x 2352 x 992 7.6 and 7.9). What is left at 16 x 12288 x 4096: 12.4 us, of which HBM needs 7.8 for the
 // weight and the launch, the first loads and the drain some 3.5 (9.6 us with the weight in L2). Tiles of fewer outputs on more SMs take as long.
 template <int T, bool kQuantize>
 struct SmallShape {
@@ -213,7 +215,7 @@ struct SmallShape {
     static constexpr int kRaw = T + 4;                                   // floats: T token scales, the weight's, padding
     static constexpr int kRawOff = kStages * kStageBytes;
     static constexpr int kBatch = kSlots / 2;                            // steps that a scale warp does at a time
-    static constexpr int kRawRing = kQuantize ? 0 : 4 * kScaleWarps * kBatch * kDeep;   // k blocks, a warp's fetched two batches ahead
+    static constexpr int kRawRing = kQuantize ? 1 : 4 * kScaleWarps * kBatch * kDeep;   // k blocks, a warp's fetched two batches ahead
     static constexpr int kProducts = 2 * kSlots * kDeep;                 // k blocks whose products are kept
     static constexpr int kScaleOff = kRawOff + kRawRing * kRaw * 4;      // [kProducts][T]
     static constexpr int kBarOff = kScaleOff + kProducts * T * 4;
@@ -558,11 +560,12 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
 // What bounds it is the way of an accumulator from the tensor core through the epilogue's registers and back to the tensor
 // core once per 128-deep block. So a k block's product is two UMMA groups of half the tile's outputs (h = 0, 1: rows
 // h * seg .. of both CTAs' weight boxes), each with two accumulators, barriers and four epilogue warps of its own: the warps of one
-// half load accumulators from tensor memory while those of the other scale theirs. A k block takes some 965 clocks of which the
-// tensor core works 512 (52 % of the active cycles at 4096 x 4096 x 4096): from the UMMAs of a half to their commit seen 600 to 770
-// behind those of the other half, loaded, scaled and released 640 to 710, seen by the issuer 250 to 330 later, for two accumulators
-// in turn. Finer groups do not help: four of 64 outputs, released at half the time, take 5 % longer (4096 x 4096 x 4096 85.3 against
-// 81.1 us, twice the barriers), 16 epilogue warps 18 % (90.3 against 76.4: half the registers, so loads and products take turns).
+// half load accumulators from tensor memory while those of the other scale theirs. A k block takes some 700
+// clocks, and the tensor core works 62 % of them (4096 x 4096 x 4096): UMMAs and commit behind those of the other half, load, scale and release by the
+// epilogue, and the issuer's wait form a ring of two accumulators. At 4096 x 4096 x 4096 (64.5 us) a quarter of the UMMAs would save 8 us, no
+// loads 7, no scaling 5, all three together 15. Finer groups do not help: four of 64 outputs, released at half the time, take 5 % longer (twice
+// the barriers), 16 epilogue warps 18 % (half the registers, so loads and products take turns), tiles of 128 outputs with four
+// accumulators 40 %.
 constexpr int kPairStages = 4;
 constexpr int kPairN = 256;
 constexpr int kPairEpilogueWarps = 8;                              // [half][lane quarter]
@@ -1049,7 +1052,7 @@ struct Choice {
 template <int T, bool kBackward, bool kOutBf16, bool kQuantize>
 Choice small_choice(const Args& args) {
     constexpr double kRound = T == 16 ? 2.6 : T == 32 ? 2.8 : 5.0;
-    constexpr double kPerBlock = T == 16 ? 0.29 : T == 32 ? 0.36 : 0.37;
+    constexpr double kPerBlock = T == 16 ? 0.28 : T == 32 ? 0.33 : 0.33;
     constexpr double kExchange = T == 16 ? 2.0 : 1.8;
     const int64_t num_kb = (args.depth() + kBlock - 1) / kBlock;
     const int64_t tiles = (args.M + T - 1) / T * ((args.width() + 127) / 128);
@@ -1065,18 +1068,18 @@ Choice small_choice(const Args& args) {
     return best;
 }
 
-// A round of the pair kernel's tiles, 0.46 a k block.
+// A round of the pair kernel's tiles, 0.43 a k block.
 double pair_cost(const Args& args) {
     const int64_t pairs = device_info().sm_count / 2;
     const int64_t tiles = (args.M + 255) / 256 * ((args.width() + kPairN - 1) / kPairN);
     const int64_t num_kb = (args.depth() + kBlock - 1) / kBlock;
-    return 4.2 + static_cast<double>((tiles + pairs - 1) / pairs) * (1.3 + 0.46 * static_cast<double>(num_kb));
+    return 4.2 + static_cast<double>((tiles + pairs - 1) / pairs) * (1.3 + 0.43 * static_cast<double>(num_kb));
 }
 
 // Up to 16 tokens one tile of 16. Above, the cheapest of tiles of 16 (up to 64 tokens), of 32 (up to 128), of 128 and the pair kernel. Measured
 // (us): 47 x 608 x 3888 backward 5.3 with tiles of 16 and 5.8 of 32, 26 x 10880 x 1568 13.3 and 7.8; 78 x 6016 x 640 5.2 with tiles of 32 and 6.0 of
-// 128, 64 x 5120 x 5120 13.5 and 10.9; 512 x 4096 x 4096 15.8 with tiles of 128 and 21.1 on the pair kernel, 744 x 7872 x 560 22.0 and 12.6, 1024 x 4096 x
-// 4096 33.7 and 22.2.
+// 128, 64 x 5120 x 5120 13.5 and 10.9; 512 x 4096 x 4096 14.1 with tiles of 128 and 20 on the pair kernel, 744 x 7872 x 560 22.0 and 12.6, 1024 x 4096 x
+// 4096 29 and 21 to 24.
 template <bool kBackward, bool kOutBf16>
 bool launch(const Args& args) {
     if (args.x != nullptr) return launch_small<16, kBackward, kOutBf16, true>(args, small_choice<16, kBackward, kOutBf16, true>(args).splits);
