@@ -563,9 +563,9 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
 // half load accumulators from tensor memory while those of the other scale theirs. A k block takes some 700
 // clocks, and the tensor core works 62 % of them (4096 x 4096 x 4096): UMMAs and commit behind those of the other half, load, scale and release by the
 // epilogue, and the issuer's wait form a ring of two accumulators. At 4096 x 4096 x 4096 (64.5 us) a quarter of the UMMAs would save 8 us, no
-// loads 7, no scaling 5, all three together 15. Finer groups do not help: four of 64 outputs, released at half the time, take 5 % longer (twice
-// the barriers), 16 epilogue warps 18 % (half the registers, so loads and products take turns), tiles of 128 outputs with four
-// accumulators 40 %.
+// loads 7, no scaling 5, all three together 15. Other groups: four of 64 outputs take 16 to 24 % longer (8192 x 12288 x 4096 486 us, 390
+// with two), one of 256 with one issuer 13 to 25 % (486). 16 epilogue warps: 18 % (half the registers, so loads and products take turns).
+// Tiles of 128 outputs with four accumulators: 40 %.
 constexpr int kPairStages = 4;
 constexpr int kPairN = 256;
 constexpr int kPairEpilogueWarps = 8;                              // [half][lane quarter]

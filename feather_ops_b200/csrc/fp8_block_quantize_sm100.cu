@@ -14,7 +14,7 @@
 // elements per clock and issues 4 warp instructions, i.e. 10 to 30 instructions per element. A thread has 8 consecutive channels
 // (one 16-byte load, one 8-byte store of codes) as four float pairs for the packed fp32 arithmetic; 16 lanes hold one block, and
 // its maximum is four shuffles. Measured, inputs from HBM: quantizer 4096 x 12288 24.4 us (6.2 TB/s of 6.46 that a copy reaches), gate
-// 4096 x 12288 39.2 (6.4), its backward pass 73.4 (6.9), norm 8192 x 4096 with a residual 38.5 (6.1), its backward pass 52.7 (5.1).
+// 4096 x 12288 39.2 (6.4), its backward pass 73.4 (6.9), norm 8192 x 4096 with a residual 38.5 (6.1), its backward pass 50.4 (5.3).
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -275,9 +275,10 @@ struct NormGradParams {
 // n = x rstd, u = grad w:  dx = rstd (u - n mean(u n)) + grad_residual,  dw = sum over rows of grad n.
 // A persistent grid: every CTA walks its rows and keeps its share of dw in registers, so that dw costs one row of partials per
 // CTA; a second kernel adds those in CTA order (the same bits on every run). A row is a chain of latencies (loads, ten shuffles, a
-// barrier), so what counts is how many rows an SM has at once: at 64 registers four CTAs of 256 threads. (Copying the next rows to
-// shared memory ahead of time was slower at the two or three CTAs that fit then: 68 to 75 us at 8192 x 4096 with a residual.)
-template <bool kFp16, bool kWeightF32, int kChunks, int kThreads>
+// barrier), so what counts is how many rows an SM has on their way: two per CTA with the next row in registers (kAhead), else, at 64 registers, four CTAs
+// of 256 threads. (Copying the next rows to shared memory ahead of time was slower at the two or three CTAs that fit then: 68 to 75 us at
+// 8192 x 4096 with a residual, and so was every variant whose registers spill.)
+template <bool kFp16, bool kWeightF32, int kChunks, int kThreads, bool kAhead>
 __global__ void __launch_bounds__(kThreads) rms_norm_dgrad_kernel(const NormGradParams p) {
     __shared__ float slots[2][32];
     extern __shared__ float total[];   // the width, with several rows per CTA
@@ -292,20 +293,41 @@ __global__ void __launch_bounds__(kThreads) rms_norm_dgrad_kernel(const NormGrad
         for (int i = 0; i < 4; ++i) dw[c][i] = both(0.0f);
     }
     bool odd = false;
-    for (int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; row < p.M; row += row_step) {
-        const int64_t base = row * p.K;
-        const float rstd = __ldg(p.rstd + row);
+    struct Row {
         uint4 x[kChunks], g[kChunks], res[kChunks];
+        float rstd;
+    };
+    const auto load = [&](int64_t row, Row& r) {
+        const bool live = row < p.M;
+        const int64_t base = row * p.K;
+        r.rstd = live ? __ldg(p.rstd + row) : 0.0f;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
             const int column = column0 + c * step;
-            x[c] = g[c] = res[c] = make_uint4(0, 0, 0, 0);
-            if (column < width) {
-                x[c] = load16(p.x + base + column);
-                g[c] = load16(p.grad + base + column);
-                if (p.grad_residual != nullptr) res[c] = load16(p.grad_residual + base + column);
+            r.x[c] = r.g[c] = r.res[c] = make_uint4(0, 0, 0, 0);
+            if (live && column < width) {
+                r.x[c] = load16(p.x + base + column);
+                r.g[c] = load16(p.grad + base + column);
+                if (p.grad_residual != nullptr) r.res[c] = load16(p.grad_residual + base + column);
             }
         }
+    };
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+    Row ahead;
+    if constexpr (kAhead) load(row0, ahead);
+    for (int64_t row = row0; row < p.M; row += row_step) {
+        Row now;
+        if constexpr (kAhead) {
+            now = ahead;
+            load(row + row_step, ahead);
+        } else {
+            load(row, now);
+        }
+        const int64_t base = row * p.K;
+        const float rstd = now.rstd;
+        const uint4(&x)[kChunks] = now.x;
+        const uint4(&g)[kChunks] = now.g;
+        const uint4(&res)[kChunks] = now.res;
         float2 dots = both(0.0f);
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
@@ -509,11 +531,22 @@ RowShape row_shape(int64_t M, int64_t K) {
     return {static_cast<int>((threads + 31) / 32 * 32), 1, chunks};
 }
 
-// CTAs of the norm's backward pass: what an SM holds at 64 registers a thread (twice that with four chunks per warp), four at most, and two
-// rows each at least.
+// The norm's backward pass has a row's successor on its way in registers (128 a thread, so 512 threads on an SM) where a row is a CTA's and those
+// CTAs leave no more than a quarter of the 512 threads unused. Measured (us, with a residual; without the next row): 20000 x 1280 46.0 (69.5), 8192 x
+// 2048 30.2 (38.6), 8192 x 4096 50.4 (52.9), 4096 x 6144 43.3 (46.7), 4096 x 8192 50.3 (54.5); 8192 x 5120, 320 threads, 73.0 (64.8); rows of a warp 20000 x 1024
+// 40.4 (37.3), 20000 x 256 15.6 (14.7).
+constexpr int kAheadThreads = 512;
+
+bool next_row_ahead(const RowShape& shape) {
+    return shape.rows == 1 && shape.chunks == 2 && shape.threads <= kAheadThreads && kAheadThreads / shape.threads * shape.threads >= kAheadThreads / 4 * 3;
+}
+
+// CTAs of the norm's backward pass: what an SM holds (without the next row: at 64 registers a thread, twice that with four chunks per warp; four at
+// most), and two rows each at least.
 int norm_grad_grid(int64_t M, const RowShape& shape) {
-    int64_t per_sm = 1024 / (shape.threads * shape.rows);
-    per_sm = per_sm > 4 ? 4 : per_sm < 1 ? 1 : per_sm;
+    int64_t per_sm = (next_row_ahead(shape) ? kAheadThreads : 1024) / (shape.threads * shape.rows);
+    if (!next_row_ahead(shape) && per_sm > 4) per_sm = 4;
+    if (per_sm < 1) per_sm = 1;
     if (shape.rows > 1 && shape.chunks == 4) per_sm = 2;
     const int64_t wanted = (M + 2 * shape.rows - 1) / (2 * shape.rows);
     return static_cast<int>(wanted < kSms * per_sm ? wanted : kSms * per_sm);
@@ -565,10 +598,11 @@ bool launch_norm_grad(const NormGradParams& p, float* grad_weight, cudaStream_t 
     }
     const RowShape shape = row_shape(p.M, p.K);
     const int grid = norm_grad_grid(p.M, shape);
-    const auto kernel = shape.chunks == 1   ? rms_norm_dgrad_kernel<kFp16, kWeightF32, 1, kMaxNormThreads>
-                        : shape.chunks == 2 ? rms_norm_dgrad_kernel<kFp16, kWeightF32, 2, kMaxNormThreads>
-                        : shape.rows > 1    ? rms_norm_dgrad_kernel<kFp16, kWeightF32, 4, 32 * kRowsPerCta>
-                                            : rms_norm_dgrad_kernel<kFp16, kWeightF32, 4, kMaxNormThreads>;
+    const auto kernel = next_row_ahead(shape) ? rms_norm_dgrad_kernel<kFp16, kWeightF32, 2, kAheadThreads, true>
+                        : shape.chunks == 1   ? rms_norm_dgrad_kernel<kFp16, kWeightF32, 1, kMaxNormThreads, false>
+                        : shape.chunks == 2   ? rms_norm_dgrad_kernel<kFp16, kWeightF32, 2, kMaxNormThreads, false>
+                        : shape.rows > 1      ? rms_norm_dgrad_kernel<kFp16, kWeightF32, 4, 32 * kRowsPerCta, false>
+                                              : rms_norm_dgrad_kernel<kFp16, kWeightF32, 4, kMaxNormThreads, false>;
     const size_t smem = shape.rows > 1 ? static_cast<size_t>(p.K) * 4 : 0;
     // An ordinary launch: a persistent grid that starts among the CTAs of the kernel ahead is spread unevenly over the SMs (84 against 68 us
     // at 8192 x 4096).

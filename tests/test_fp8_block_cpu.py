@@ -82,8 +82,8 @@ def test_launchers_refuse_bad_arguments_without_a_device(lib):
 
 
 def test_scratch_of_the_norms_weight_gradient(lib):
-    # few rows: none. Else a row of partials per CTA: two rows of the input each at least, and at most four CTAs per SM
-    for m, k, ctas in ((0, 272, 0), (1, 272, 0), (1024, 8192, 0), (512, 496, 0), (513, 496, 33), (1025, 4096, 513), (100, 16384, 50), (100000, 2048, 592), (100000, 4096, 592), (100000, 32768, 148), (100000, 8192, 296), (100000, 512, 592)):
+    # few rows: none. Else a row of partials per CTA: two rows of the input each at least, and no more CTAs than the SMs hold
+    for m, k, ctas in ((0, 272, 0), (1, 272, 0), (1024, 8192, 0), (512, 496, 0), (513, 496, 33), (1025, 4096, 296), (100, 16384, 50), (100000, 2048, 592), (100000, 4096, 296), (100000, 1296, 740), (100000, 5120, 444), (100000, 32768, 148), (100000, 8192, 148), (100000, 512, 592)):
         assert lib.feather_rms_norm_dgrad_partial_floats(m, k) == ctas * k
 
 

@@ -232,6 +232,14 @@ def test_norm_gradients(cuda_device, shape, x_type, w_type, residual):
     assert torch.equal(again[0], gx) and torch.equal(again[1], gw)
 
 
+# Many rows of a CTA each: with the next row in registers and (5120 channels) without; one to three rows per CTA, and CTAs that end early.
+@pytest.mark.parametrize("residual", [False, True], ids=["plain", "residual"])
+@pytest.mark.parametrize("x_type,w_type", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32)])
+@pytest.mark.parametrize("shape", [(1025, 4096), (1100, 1040), (1300, 2576), (1111, 6160), (1030, 8192), (1027, 5120), (3001, 1296)], ids=lambda s: "x".join(map(str, s)))
+def test_norm_gradients_of_many_rows(cuda_device, shape, x_type, w_type, residual):
+    test_norm_gradients(cuda_device, shape, x_type, w_type, residual)
+
+
 def test_norm_of_no_rows(cuda_device):
     x = torch.empty(0, 256, device=cuda_device, dtype=torch.bfloat16)
     w = torch.ones(256, device=cuda_device, dtype=torch.bfloat16)
