@@ -1098,16 +1098,16 @@ bool launch(const Args& args) {
     return launch_pair<kBackward, kOutBf16>(args);
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 bool valid(const Args& args) {
     constexpr int64_t kMost = 1 << 30;
     if (args.M < 0 || args.N <= 0 || args.K <= 0 || args.M > kMost || args.N > kMost || args.K > kMost || args.N % 16 != 0 || args.K % 16 != 0) return false;
     if (args.transposed_b && args.bias != nullptr) return false;
     if (args.M == 0) return true;
-    const bool codes = args.a != nullptr && args.a_scale != nullptr && aligned16(args.a);
-    if (!(args.x != nullptr ? aligned16(args.x) : codes) || args.w == nullptr || args.w_scale == nullptr || args.c == nullptr) return false;
-    return aligned16(args.w) && aligned16(args.c);
+    const bool codes = args.a != nullptr && args.a_scale != nullptr && aligned(args.a, 16) && aligned(args.a_scale, 4);
+    if (!(args.x != nullptr ? aligned(args.x, 16) : codes) || args.w == nullptr || args.w_scale == nullptr || args.c == nullptr) return false;
+    return aligned(args.w, 16) && aligned(args.c, 16) && aligned(args.w_scale, 4) && aligned(args.bias, 2);
 }
 
 bool launch(const Args& args) {

@@ -650,7 +650,7 @@ extern "C" bool launch_rms_norm_fp8(const void* x, const void* residual, const v
     if (M < 0 || M > 0x7fffffff || K <= 0 || K % 16 != 0 || K > kMaxNormWidth) return false;
     if (M == 0) return true;
     if (x == nullptr || weight == nullptr || q == nullptr || scale == nullptr || rstd == nullptr || (residual == nullptr) != (residual_out == nullptr)) return false;
-    if (!aligned(x, 16) || !aligned(residual, 16) || !aligned(weight, 16) || !aligned(residual_out, 16) || !aligned(q, 16)) return false;
+    if (!aligned(x, 16) || !aligned(residual, 16) || !aligned(weight, 16) || !aligned(residual_out, 16) || !aligned(q, 16) || !aligned(scale, 4) || !aligned(rstd, 4)) return false;
     const NormParams p{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(residual), weight, static_cast<uint16_t*>(residual_out),
                        static_cast<uint8_t*>(q), scale, rstd, M, K, eps};
     switch ((input_fp16 != 0 ? 4 : 0) | (weight_f32 != 0 ? 2 : 0) | (use_e5m2 != 0 ? 1 : 0)) {
@@ -674,7 +674,7 @@ extern "C" bool launch_rms_norm_dgrad(const void* grad, const void* x, const voi
                                       float* grad_weight, float* partials, int64_t M, int64_t K, int input_fp16, int weight_f32, cudaStream_t stream) {
     if (M <= 0 || M > 0x7fffffff || K <= 0 || K % 16 != 0 || K > kMaxNormWidth) return false;
     if (grad == nullptr || x == nullptr || weight == nullptr || rstd == nullptr || grad_x == nullptr || grad_weight == nullptr || (partials == nullptr && !few_rows(M, K))) return false;
-    if (!aligned(grad, 16) || !aligned(x, 16) || !aligned(weight, 16) || !aligned(grad_residual, 16) || !aligned(grad_x, 16) || !aligned(grad_weight, 8) || !aligned(partials, 16)) return false;
+    if (!aligned(grad, 16) || !aligned(x, 16) || !aligned(weight, 16) || !aligned(grad_residual, 16) || !aligned(grad_x, 16) || !aligned(grad_weight, 8) || !aligned(partials, 16) || !aligned(rstd, 4)) return false;
     const NormGradParams p{static_cast<const uint16_t*>(grad), static_cast<const uint16_t*>(x), weight, rstd, static_cast<const uint16_t*>(grad_residual),
                            static_cast<uint16_t*>(grad_x), partials, M, K};
     if (input_fp16 != 0) {

@@ -81,6 +81,21 @@ def test_launchers_refuse_bad_arguments_without_a_device(lib):
     assert not lib.launch_silu_mul_dgrad(p, p, None, 4, 16, 0, None)
 
 
+def test_launchers_refuse_scales_off_their_alignment(lib):
+    p = 1 << 20  # never dereferenced: every call below is refused
+    assert not lib.launch_fp8_block_mm(p, p + 2, p, p, None, p, 4, 32, 32, False, 0, 0, 1, None)
+    assert not lib.launch_fp8_block_mm(p, p, p, p + 1, None, p, 4, 32, 32, False, 0, 0, 1, None)
+    assert not lib.launch_fp8_block_mm(p, p, p, p, p + 1, p, 4, 32, 32, False, 0, 0, 1, None)
+    assert not lib.launch_fp8_block_linear(p, None, p, p + 2, None, p, 4, 32, 32, False, 0, 0, 0, 1, None)
+    assert not lib.launch_fp8_block_linear(p, p + 8, p, p, None, p, 40, 32, 32, False, 0, 0, 0, 1, None)
+    assert not lib.launch_fp8_block_linear(p, None, p, p, None, p, 40, 32, 32, False, 0, 0, 0, 1, None)
+    assert not lib.launch_fp8_block_quantize(p, p, p + 2, 4, 32, 0, 0, None)
+    assert not lib.launch_rms_norm_fp8(p, None, p, None, p, p + 2, p, 4, 32, 1e-6, 0, 0, 0, None)
+    assert not lib.launch_rms_norm_fp8(p, None, p, None, p, p, p + 2, 4, 32, 1e-6, 0, 0, 0, None)
+    assert not lib.launch_rms_norm_dgrad(p, p, p, p + 2, None, p, p, p, 4, 32, 0, 0, None)
+    assert not lib.launch_rms_norm_dgrad(p, p, p, p, None, p, p + 4, p, 4, 32, 0, 0, None)
+
+
 def test_scratch_of_the_norms_weight_gradient(lib):
     # few rows: none. Else a row of partials per CTA: two rows of the input each at least, and no more CTAs than the SMs hold
     for m, k, ctas in ((0, 272, 0), (1, 272, 0), (1024, 8192, 0), (512, 496, 0), (513, 496, 33), (1025, 4096, 296), (100, 16384, 50), (100000, 2048, 592), (100000, 4096, 296), (100000, 1296, 740), (100000, 5120, 444), (100000, 32768, 148), (100000, 8192, 148), (100000, 512, 592)):
