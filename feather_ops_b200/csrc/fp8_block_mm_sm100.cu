@@ -565,7 +565,7 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
 // epilogue, and the issuer's wait form a ring of two accumulators. At 4096 x 4096 x 4096 (64.5 us) a quarter of the UMMAs would save 8 us, no
 // loads 7, no scaling 5, all three together 15. Other groups: four of 64 outputs take 16 to 24 % longer (8192 x 12288 x 4096 486 us, 390
 // with two), one of 256 with one issuer 13 to 25 % (486). 16 epilogue warps: 18 % (half the registers, so loads and products take turns).
-// Tiles of 128 outputs with four accumulators: 40 %.
+// Tiles of 128 outputs with four accumulators: 25 % (82.3 against 65.7), and slower than small_kernel where that is picked (512 x 4096 x 4096 16.0, 14.0).
 constexpr int kPairStages = 4;
 constexpr int kPairN = 256;
 constexpr int kPairEpilogueWarps = 8;                              // [half][lane quarter]
