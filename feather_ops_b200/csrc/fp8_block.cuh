@@ -8,6 +8,8 @@
 
 #include <cstdint>
 
+#include "sm100_ptx.cuh"
+
 namespace feather {
 namespace f8 {
 
@@ -103,7 +105,11 @@ __device__ __forceinline__ uint2 encode_block(const Pairs& v, float top, float& 
     return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
 }
 
-__device__ __forceinline__ uint4 load16(const uint16_t* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+// 16 bytes of an input, by a kernel that may start before the one ahead has finished writing them
+__device__ __forceinline__ uint4 load16(const uint16_t* p) { return ld_global_v4(p); }
+
+// ... by an ordinary launch
+__device__ __forceinline__ uint4 load16_readonly(const uint16_t* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
 
 }  // namespace f8
 }  // namespace feather

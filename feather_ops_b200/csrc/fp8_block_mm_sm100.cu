@@ -353,7 +353,7 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
         const auto fetch = [&](int i) {
             if (i >= blocks) return;
             const int column = (kb_begin + i) * kBlock;
-            sw = __ldg(w_scale + i * p.w_scale_block);
+            sw = ld_global_f32(w_scale + i * p.w_scale_block);
 #pragma unroll
             for (int t = 0; t < kQuantizePasses; ++t) {
                 const int token = 2 * t + lane / 16;
@@ -523,7 +523,7 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
         float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         if (p.bias != nullptr) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) bias[j] = bits_to_float<kOutBf16>(__ldg(p.bias + column + j));
+            for (int j = 0; j < 4; ++j) bias[j] = bits_to_float<kOutBf16>(ld_global_u16(p.bias + column + j));
         }
         for (int t = rank * share + warp; t < token_end; t += L::kThreads / 32) {
             float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -821,13 +821,13 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
                 const int column = chunk_column(col0, c);
-                if (p.bias != nullptr && column < p.width) {
+                if (p.bias != nullptr) {
+                    // a lane loads one output's, and hands it to the others
+                    const float bias = column + lane < p.width ? bits_to_float<kOutBf16>(ld_global_u16(p.bias + column + lane)) : 0.0f;
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
-                        if (column + 2 * j < p.width) {
-                            acc[c][j].x += bits_to_float<kOutBf16>(__ldg(p.bias + column + 2 * j));
-                            acc[c][j].y += bits_to_float<kOutBf16>(__ldg(p.bias + column + 2 * j + 1));
-                        }
+                        acc[c][j].x += __shfl_sync(0xffffffffu, bias, 2 * j);
+                        acc[c][j].y += __shfl_sync(0xffffffffu, bias, 2 * j + 1);
                     }
                 }
 #pragma unroll

@@ -58,8 +58,8 @@ __device__ __forceinline__ float2 sigmoid(float2 x) {
 constexpr int kTileWarps = 8;
 
 template <bool kFp16, bool kE5M2, bool kGate, int kRows>
-__global__ void __launch_bounds__(32 * kTileWarps) tile_quantize_kernel(const uint16_t* __restrict__ x, uint8_t* __restrict__ q,
-                                                                        float* __restrict__ scale, int64_t M, int64_t K, int column_warps) {
+__global__ void __launch_bounds__(32 * kTileWarps) tile_quantize_kernel(const uint16_t* x, uint8_t* q,
+                                                                        float* scale, int64_t M, int64_t K, int column_warps) {
     start_after_kernel_ahead();
     const int lane = threadIdx.x & 31;
     const int64_t task = static_cast<int64_t>(blockIdx.x) * kTileWarps + (threadIdx.x >> 5);
@@ -100,8 +100,8 @@ __global__ void __launch_bounds__(32 * kTileWarps) tile_quantize_kernel(const ui
 
 // d/dgate = g u s (1 + gate (1 - s)), d/dup = g gate s, with s = sigmoid(gate).
 template <bool kFp16>
-__global__ void __launch_bounds__(256) silu_mul_dgrad_kernel(const uint16_t* __restrict__ grad, const uint16_t* __restrict__ gate_up,
-                                                             uint16_t* __restrict__ out, int64_t chunks, int64_t row_chunks) {
+__global__ void __launch_bounds__(256) silu_mul_dgrad_kernel(const uint16_t* grad, const uint16_t* gate_up,
+                                                             uint16_t* out, int64_t chunks, int64_t row_chunks) {
     start_after_kernel_ahead();
     const int64_t chunk = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     if (chunk >= chunks) return;
@@ -152,15 +152,17 @@ __device__ __forceinline__ float row_sum(float v, float* slots) {
     return v;
 }
 
-template <bool kFp16, bool kWeightF32>
+// kReadonly: by an ordinary launch (see load16_readonly)
+template <bool kFp16, bool kWeightF32, bool kReadonly>
 __device__ __forceinline__ void load_weight(const void* weight, int64_t column, Pairs& w) {
+    const auto load = [](const uint16_t* p) { return kReadonly ? load16_readonly(p) : load16(p); };
     if constexpr (kWeightF32) {
-        const float4* const p = reinterpret_cast<const float4*>(static_cast<const float*>(weight) + column);
-        const float4 lo = __ldg(p), hi = __ldg(p + 1);
-        w[0] = make_float2(lo.x, lo.y), w[1] = make_float2(lo.z, lo.w);
-        w[2] = make_float2(hi.x, hi.y), w[3] = make_float2(hi.z, hi.w);
+        const uint16_t* const p = reinterpret_cast<const uint16_t*>(static_cast<const float*>(weight) + column);
+        const uint4 lo = load(p), hi = load(p + 8);
+        w[0] = make_float2(__uint_as_float(lo.x), __uint_as_float(lo.y)), w[1] = make_float2(__uint_as_float(lo.z), __uint_as_float(lo.w));
+        w[2] = make_float2(__uint_as_float(hi.x), __uint_as_float(hi.y)), w[3] = make_float2(__uint_as_float(hi.z), __uint_as_float(hi.w));
     } else {
-        unpack8<kFp16>(load16(static_cast<const uint16_t*>(weight) + column), w);
+        unpack8<kFp16>(load(static_cast<const uint16_t*>(weight) + column), w);
     }
 }
 
@@ -244,7 +246,7 @@ __global__ void __launch_bounds__(kMaxNormThreads) rms_norm_fp8_kernel(const Nor
         const int column = column0 + c * step;
         const bool live = column < width;
         Pairs w = {};
-        if (live) load_weight<kFp16, kWeightF32>(p.weight, column, w);
+        if (live) load_weight<kFp16, kWeightF32, false>(p.weight, column, w);
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
             Pairs v;
@@ -306,9 +308,9 @@ __global__ void __launch_bounds__(kThreads) rms_norm_dgrad_kernel(const NormGrad
             const int column = column0 + c * step;
             r.x[c] = r.g[c] = r.res[c] = make_uint4(0, 0, 0, 0);
             if (live && column < width) {
-                r.x[c] = load16(p.x + base + column);
-                r.g[c] = load16(p.grad + base + column);
-                if (p.grad_residual != nullptr) r.res[c] = load16(p.grad_residual + base + column);
+                r.x[c] = load16_readonly(p.x + base + column);
+                r.g[c] = load16_readonly(p.grad + base + column);
+                if (p.grad_residual != nullptr) r.res[c] = load16_readonly(p.grad_residual + base + column);
             }
         }
     };
@@ -336,7 +338,7 @@ __global__ void __launch_bounds__(kThreads) rms_norm_dgrad_kernel(const NormGrad
                 Pairs n, u, w;
                 unpack8<kFp16>(x[c], n);
                 unpack8<kFp16>(g[c], u);
-                load_weight<kFp16, kWeightF32>(p.weight, column, w);
+                load_weight<kFp16, kWeightF32, true>(p.weight, column, w);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     n[i] = __fmul2_rn(n[i], both(rstd));
@@ -356,7 +358,7 @@ __global__ void __launch_bounds__(kThreads) rms_norm_dgrad_kernel(const NormGrad
                 unpack8<kFp16>(x[c], n);
                 unpack8<kFp16>(g[c], u);
                 unpack8<kFp16>(res[c], r);
-                load_weight<kFp16, kWeightF32>(p.weight, column, w);
+                load_weight<kFp16, kWeightF32, true>(p.weight, column, w);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) r[i] = __ffma2_rn(n[i], back, __ffma2_rn(__fmul2_rn(u[i], w[i]), both(rstd), r[i]));
                 *reinterpret_cast<uint4*>(p.grad_x + base + column) = pack8<kFp16>(r);
@@ -407,7 +409,7 @@ constexpr int kFewThreads = 512;                    // at least, for the channel
 constexpr int kColumnTile = 64;
 
 template <bool kFp16, bool kWeightF32>
-__global__ void __launch_bounds__(kMaxNormThreads) rms_norm_dgrad_few_kernel(const NormGradParams p, float* __restrict__ grad_weight) {
+__global__ void __launch_bounds__(kMaxNormThreads) rms_norm_dgrad_few_kernel(const NormGradParams p, float* grad_weight) {
     __shared__ float slots[32];
     __shared__ float2 sums[32][kColumnTile / 2];
     start_after_kernel_ahead();
@@ -417,7 +419,7 @@ __global__ void __launch_bounds__(kMaxNormThreads) rms_norm_dgrad_few_kernel(con
         const int64_t row = blockIdx.x;
         const int column = threadIdx.x * kVec;
         const bool live = column < width;
-        const float rstd = __ldg(p.rstd + row);
+        const float rstd = ld_global_f32(p.rstd + row);
         Pairs n = {}, u = {}, r = {};
         float2 dots = both(0.0f);
         if (live) {
@@ -425,7 +427,7 @@ __global__ void __launch_bounds__(kMaxNormThreads) rms_norm_dgrad_few_kernel(con
             unpack8<kFp16>(load16(p.x + row * p.K + column), n);
             unpack8<kFp16>(load16(p.grad + row * p.K + column), u);
             if (p.grad_residual != nullptr) unpack8<kFp16>(load16(p.grad_residual + row * p.K + column), r);
-            load_weight<kFp16, kWeightF32>(p.weight, column, w);
+            load_weight<kFp16, kWeightF32, false>(p.weight, column, w);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 n[i] = __fmul2_rn(n[i], both(rstd));
@@ -450,7 +452,7 @@ __global__ void __launch_bounds__(kMaxNormThreads) rms_norm_dgrad_few_kernel(con
             Pairs n, g;
             unpack8<kFp16>(load16(p.x + static_cast<int64_t>(row) * p.K + column), n);
             unpack8<kFp16>(load16(p.grad + static_cast<int64_t>(row) * p.K + column), g);
-            const float2 rstd = both(__ldg(p.rstd + row));
+            const float2 rstd = both(ld_global_f32(p.rstd + row));
 #pragma unroll
             for (int i = 0; i < 4; ++i) sum[i] = __ffma2_rn(g[i], __fmul2_rn(n[i], rstd), sum[i]);
         }
@@ -476,7 +478,7 @@ __global__ void __launch_bounds__(kMaxNormThreads) rms_norm_dgrad_few_kernel(con
 
 // out[k] = sum over the rows of partials, row groups first (one per warp), then the groups in order.
 constexpr int kSumWarps = 8;
-__global__ void __launch_bounds__(32 * kSumWarps) column_sum_kernel(const float* __restrict__ partials, float* __restrict__ out, int rows, int64_t K) {
+__global__ void __launch_bounds__(32 * kSumWarps) column_sum_kernel(const float* partials, float* out, int rows, int64_t K) {
     __shared__ float part[kSumWarps][33];
     grid_dependency_wait();   // launched behind the kernel that writes the partials, as its dependent
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -484,7 +486,7 @@ __global__ void __launch_bounds__(32 * kSumWarps) column_sum_kernel(const float*
     float sum = 0.0f;
     if (column < K) {
 #pragma unroll 8
-        for (int r = warp; r < rows; r += kSumWarps) sum += partials[r * K + column];
+        for (int r = warp; r < rows; r += kSumWarps) sum += ld_global_f32(partials + r * K + column);
     }
     part[warp][lane] = sum;
     __syncthreads();

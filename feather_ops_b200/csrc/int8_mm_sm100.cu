@@ -670,8 +670,8 @@ int8_mm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 for (int i = 0; i < 8 / kEpiWarps; ++i) {
                     const int c = kPlainB ? epi_warp * 32 + lane : quarter * 64 + i * 32 + lane;
                     const int col = n0 + c;
-                    col_scale[c] = has_scale && col < p.N_out ? __ldg(p.b_scale + col) : 1.0f;
-                    col_bias[c] = has_bias && col < p.N_out ? out_bits_to_float<kOutBf16>(__ldg(p.bias + col)) : 0.0f;
+                    col_scale[c] = has_scale && col < p.N_out ? ld_global_f32(p.b_scale + col) : 1.0f;
+                    col_bias[c] = has_bias && col < p.N_out ? out_bits_to_float<kOutBf16>(ld_global_u16(p.bias + col)) : 0.0f;
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&columns_full[acc.idx]);
@@ -682,7 +682,7 @@ int8_mm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             if (!ok) break;
             tc_fence_after_sync();
             const int row = m0 + quarter * 32 + lane;
-            const float row_scale = row < p.M ? __ldg(p.a_scale + row) : 0.0f;
+            const float row_scale = row < p.M ? ld_global_f32(p.a_scale + row) : 0.0f;
             const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc.idx * kPairN;
             uint16_t* const c_row = p.c + static_cast<int64_t>(row) * p.N_out;
 #pragma unroll 1

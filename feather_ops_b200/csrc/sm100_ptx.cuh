@@ -124,6 +124,25 @@ struct WaitGuard {
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// Loads for such kernels of what the kernel ahead may still be writing when this one starts. The read-only path (__ldg, or a `const
+// __restrict__` parameter) is for data that nobody writes while the kernel is resident, and the compiler may move such a load above
+// the wait; these are ordinary loads and stay where they stand.
+__device__ __forceinline__ uint4 ld_global_v4(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(__cvta_generic_to_global(p)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float ld_global_f32(const float* p) {
+    float v;
+    asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(__cvta_generic_to_global(p)) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint16_t ld_global_u16(const uint16_t* p) {
+    uint16_t v;
+    asm volatile("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(__cvta_generic_to_global(p)) : "memory");
+    return v;
+}
+
 // Generic-proxy writes to shared memory (st.shared) -> visible to the async proxy (UMMA, TMA stores).
 __device__ __forceinline__ void fence_proxy_async_smem() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
