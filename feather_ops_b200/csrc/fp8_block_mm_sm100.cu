@@ -416,10 +416,15 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
         for (int i0 = first; i0 < steps; i0 += kTurn) {
             cp_async_wait<1>();
             __syncwarp();
-            // The slots' previous products are complete (they come in order, so the last one's is enough): these arrivals
+            // Every slot's previous products are complete (nothing orders the arrivals of two commits): these arrivals
             // count for the next ones, and the scales of two turns ago, which stood where these go, have been read.
-            const int before = i0 + kBatch - 1 - L::kSlots;
-            if (before >= 0 && !warp_wait(guard, &tmem_full[before % L::kSlots], static_cast<uint32_t>(before / L::kSlots) & 1u, kSiteTmemFull)) break;
+            bool complete = true;
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) {
+                const int before = i0 + j - L::kSlots;
+                if (before >= 0 && complete) complete = warp_wait(guard, &tmem_full[before % L::kSlots], static_cast<uint32_t>(before / L::kSlots) & 1u, kSiteTmemFull);
+            }
+            if (!complete) break;
 #pragma unroll
             for (int j = 0; j < kFetch; ++j) {
                 const int at = i0 * kDeep + j;
