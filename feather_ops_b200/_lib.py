@@ -66,6 +66,7 @@ PROTOTYPES = {
     "feather_rms_norm_dgrad_partial_floats": (_i64, [_i64, _i64]),
     "launch_silu_mul_fp8": (_c_bool, [_ptr, _ptr, _ptr, _i64, _i64, _c_int, _c_int, _ptr]),
     "launch_silu_mul_dgrad": (_c_bool, [_ptr, _ptr, _ptr, _i64, _i64, _c_int, _ptr]),
+    "feather_selftest_late_writer": (_c_int, [_ptr, _ptr, _i64, ctypes.c_longlong, _ptr]),
     "feather_selftest_wait_runs_out": (_c_int, [ctypes.c_longlong, _ptr, _ptr, _ptr]),
 }
 

@@ -317,6 +317,7 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
     } else if (warp == L::kWarps + 1) {
         // ---------------------------------------------------------------------- multiplies
         if (elect_one()) {
+            grid_dependency_wait();
             Ring slot, out;
             for (int i = 0; i < steps; ++i) {
                 if (!guard.wait(&tmem_empty[out.idx], out.phase ^ 1u, kSiteTmemEmpty)) break;
@@ -453,6 +454,7 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
 #pragma unroll
         for (int t = 0; t < kColumns / 2; ++t) acc[t] = make_float2(0.0f, 0.0f);
         bool ok = true;
+        grid_dependency_wait();
 #pragma unroll 1
         for (int i = team; i < steps; i += L::kTeams) {
             const int at = i % L::kSlots;
@@ -669,6 +671,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             // even on a barrier that is there, takes the issuing thread 75 clocks and a group with its commits 200. (One thread for both
             // halves, which then wait for one another: 4096 x 4096 x 4096 83.7 us, 81.7 with two.)
             const int h = warp - 1;
+            grid_dependency_wait();
             Ring slot, out;
             bool ok = true;
             for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
@@ -692,6 +695,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             }
         } else if (warp == 1 && cta == 1 && elect_one()) {
             // ------------------------------------------------------------------ tells CTA 0 that this CTA's boxes have landed
+            grid_dependency_wait();
             Ring slot;
             bool ok = true;
             for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step) {

@@ -599,6 +599,7 @@ int8_mm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     } else if (warp == 1) {
         // ------------------------------------------------------------------ MMA issuer (CTA 0 of the pair)
         if (cta == 0 && elect_one()) {
+            grid_dependency_wait();
             Ring slot, operand, acc;
             bool ok = true;
             for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
@@ -771,6 +772,7 @@ int8_mm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         // ------------------------------------------------------------------ plain weight: one thread per CTA tells the MMA thread
         // (CTA 0) that this CTA's boxes of a k block have landed; the other warps of this role have nothing to do
         if (warp == kPlainRelayWarp && elect_one()) {
+            grid_dependency_wait();
             Ring slot;
             bool ok = true;
             for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
@@ -793,6 +795,7 @@ int8_mm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         const uint32_t live_groups = static_cast<uint32_t>(p.tile_n / 8);   // groups of four operand rows in this CTA's half of the tile
         Ring slot, operand;
         bool ok = true;
+        grid_dependency_wait();
         uint32_t turn = 0;  // k blocks since the start of the kernel, modulo the number of teams
         for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
             for (int kb = 0; kb < num_kb; ++kb) {

@@ -1,4 +1,5 @@
-// Self-test of the bounded device waits that every tcgen05 kernel in this library is built on.
+// Self-tests: of the bounded device waits that every tcgen05 kernel in this library is built on, and (late_writer_kernel) of the kernels that
+// may start before the one ahead of them has finished.
 //
 // The kernels never spin without a limit: a wait that runs out records where it gave up in a status word, raises
 // the CTA's abort flag and returns, so the kernel drains and exits with the context intact. That path cannot be
@@ -38,6 +39,15 @@ __global__ void __launch_bounds__(64, 1) wait_runs_out_kernel(long long limit_cy
     if (threadIdx.x == 32) observed[2] = completed ? 1u : 0u;
 }
 
+// Lets its dependents start at once and writes its output late: what a kernel that starts early has to wait for.
+__global__ void __launch_bounds__(256) late_writer_kernel(const uint16_t* src, uint16_t* dst, int64_t count, long long delay_cycles) {
+    grid_launch_dependents();
+    const long long start = clock64();
+    while (clock64() - start < delay_cycles) {
+    }
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < count; i += static_cast<int64_t>(gridDim.x) * blockDim.x) dst[i] = src[i];
+}
+
 }  // namespace selftest
 }  // namespace feather
 
@@ -64,4 +74,14 @@ extern "C" int feather_selftest_wait_runs_out(long long limit_cycles, uint32_t* 
     out[3] = seen[1];
     out[4] = seen[2];
     return 0;
+}
+
+// Copies `bytes` (a multiple of two) from `src` to `dst` on `stream`, `delay_cycles` SM clocks (clamped to [0, 6e9], three seconds) after it has let
+// the kernel behind it in the stream start. Returns 0 on success, 1 for bad arguments or a failed launch. No counterpart in the reference.
+extern "C" int feather_selftest_late_writer(const void* src, void* dst, int64_t bytes, long long delay_cycles, cudaStream_t stream) {
+    if (src == nullptr || dst == nullptr || bytes < 0 || bytes % 2 != 0 || ((reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst)) & 1) != 0) return 1;
+    if (delay_cycles < 0) delay_cycles = 0;
+    if (delay_cycles > 6000000000LL) delay_cycles = 6000000000LL;
+    feather::selftest::late_writer_kernel<<<16, 256, 0, stream>>>(static_cast<const uint16_t*>(src), static_cast<uint16_t*>(dst), bytes / 2, delay_cycles);
+    return cudaGetLastError() == cudaSuccess ? 0 : 1;
 }

@@ -120,7 +120,8 @@ struct WaitGuard {
 // Programmatic dependent launch. A kernel launched with the programmatic-stream-serialization attribute may start while the
 // kernel before it in the stream is still running; `grid_dependency_wait` returns once that kernel has completed and its
 // memory is visible (at once when the launch carries no such attribute). `grid_launch_dependents` tells the scheduler that
-// the kernel after this one may start as soon as every CTA of this one has called it or exited.
+// the kernel after this one may start as soon as every CTA of this one has called it or exited. The kernel ahead may run for longer than
+// a guarded wait lasts, so every warp calls `grid_dependency_wait` before its first one.
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
@@ -334,6 +335,11 @@ __device__ __forceinline__ uint32_t map_to_cta(uint32_t local, uint32_t rank) {
 // 16 bytes into another CTA's shared memory (distributed shared memory; the address comes from map_to_cta)
 __device__ __forceinline__ void st_shared_cluster_v4(uint32_t cluster_addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
     asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+// 4 bytes into a CTA's shared memory (this one's or a peer's)
+__device__ __forceinline__ void st_shared_cluster_u32(uint32_t cluster_addr, uint32_t x) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(x) : "memory");
 }
 
 // 16 bytes from a CTA's shared memory (this one's or a peer's)

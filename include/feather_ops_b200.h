@@ -204,6 +204,10 @@ bool launch_silu_mul_dgrad(const void* grad, const void* gate_up, void* grad_gat
  * No counterpart in the reference (its kernels have no device-side waits). */
 int feather_selftest_wait_runs_out(long long limit_cycles, uint32_t* scratch, uint32_t* out, feather_stream_t stream);
 
+/* Self-test of kernels that may start before the one ahead of them has finished: copies `bytes` (a multiple of two) from src to dst, delay_cycles SM
+ * clocks (clamped to [0, 6e9]) after it has let the kernel behind it in the stream start. Returns 0 on success. No counterpart in the reference. */
+int feather_selftest_late_writer(const void* src, void* dst, int64_t bytes, long long delay_cycles, feather_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,7 +1,8 @@
 """What the sources of kernels that may start before the kernel ahead of them has finished have to keep to.
 
 Such a kernel (programmatic dependent launch) is resident while the kernel ahead still writes its inputs. So it reads none of them through
-the read-only path, whose data nobody may write while the kernel runs and whose loads the compiler may move above the wait.
+the read-only path, whose data nobody may write while the kernel runs and whose loads the compiler may move above the wait, and none
+of its warps begins a wait that has a limit before the kernel ahead has finished, which may take longer.
 """
 
 import re
@@ -69,3 +70,25 @@ def test_inputs_are_not_read_through_the_read_only_path(name, kernel):
     text = without_comments((_build.CSRC / "fp8_block.cuh").read_text())
     load16 = re.search(r"\bload16\(const uint16_t\* p\)\s*(\{[^}]*\})", text)[1]
     assert "__ldg" not in load16
+
+
+def waits_for_the_kernel_ahead_first(body: str, at: int) -> bool:
+    """Whether the code on the way to `at` (the blocks that are open there, without those closed before) has the dependency wait."""
+    way = [""]
+    for c in body[:at]:
+        if c == "{":
+            way.append("")
+        elif c == "}":
+            way.pop()
+        else:
+            way[-1] += c
+    return any(WAITS.search(part) for part in way)
+
+
+@pytest.mark.parametrize("name,kernel", dependents())
+def test_no_limited_wait_begins_before_the_kernel_ahead_has_finished(name, kernel):
+    body = kernels(name)[kernel][1]
+    waits = [m.start() for m in re.finditer(r"\b(guard\.wait|warp_wait)\(", body)]
+    assert waits or not kernel.endswith(("small_kernel", "pair_kernel"))
+    early = [body[at : at + 70] for at in waits if not waits_for_the_kernel_ahead_first(body, at)]
+    assert not early
