@@ -520,9 +520,14 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
     }
 
     // The cluster's CTAs share the tile's tokens out and add all partial sums of theirs: split by split, team by team.
+    // One whose wait has run out has none to add, so it takes the whole cluster along, and the outputs stay unwritten.
     __syncwarp();
     __syncthreads();
-    if (splits > 1) cluster_sync_all();
+    if (splits > 1) {
+        if (warp == 0 && lane < splits && guard.aborted()) st_shared_cluster_u32(map_to_cta(smem_u32(tmem_slot + 1), static_cast<uint32_t>(lane)), 1u);
+        __syncwarp();
+        cluster_sync_all();
+    }
     const int share = (live + splits - 1) / splits;
     const int token_end = (rank + 1) * share < live ? (rank + 1) * share : live;
     const int column = n0 + 4 * lane;

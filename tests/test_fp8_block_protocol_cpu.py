@@ -81,3 +81,14 @@ def test_the_model_sees_an_early_read():
 def test_no_order_of_arrivals_lets_the_epilogue_read_early(seeds):
     waited = slots_waited_for()
     assert not any(epilogue_reads_early(waited, seed) for seed in seeds)
+
+
+def test_a_cta_that_gave_up_takes_its_cluster_along():
+    """With the contraction split over a cluster every CTA adds the partial sums of all: none may add those of a CTA whose wait has run out. The
+    abort flag is a word of the CTA's own, so it has to reach the peers before the barrier behind which they look at theirs."""
+    body = re.sub(r"\s+", " ", kernels("fp8_block_mm_sm100.cu")["small_kernel"][1])
+    assert "abort_flag = tmem_slot + 1;" in body
+    barrier, look = body.index("cluster_sync_all()"), body.index("column < p.width && !guard.aborted()")
+    told = body.find("if (warp == 0 && lane < splits && guard.aborted()) st_shared_cluster_u32(map_to_cta(smem_u32(tmem_slot + 1), static_cast<uint32_t>(lane)), 1u);")
+    assert -1 < told < barrier < look
+    assert "__syncthreads(); if (splits > 1) {" in body[told - 60 : told]   # every warp of this CTA has set the flag by then, if it does
