@@ -692,8 +692,10 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                         const uint64_t desc_w = kBackward ? make_desc_sw128_mnmajor(w_addr + k * 32 * 128) : make_desc_sw128_kmajor(w_addr + k * 32);
                         umma_f8_pair(tmem_base + out.idx * kPairN + h * kPairN / 2, make_desc_sw128_kmajor(a_addr + k * 32), desc_w, p.idesc, k != 0 ? 1u : 0u);
                     }
-                    umma_commit_pair_both(&tmem_full[2 * h + out.idx]);
-                    umma_commit_pair_both(&load_empty[slot.idx]);
+#pragma unroll
+                    for (uint32_t dst = 0; dst < 2; ++dst) umma_commit_pair(map_to_cta(smem_u32(&tmem_full[2 * h + out.idx]), dst));
+#pragma unroll
+                    for (uint32_t dst = 0; dst < 2; ++dst) umma_commit_pair(map_to_cta(smem_u32(&load_empty[slot.idx]), dst));
                     slot.advance(kPairStages);
                     out.advance(2);
                 }

@@ -185,3 +185,12 @@ def test_build_entry_loads_no_extension():
         "sys.exit('feather_ops_b200._C' in sys.modules)"
     )
     assert subprocess.run([sys.executable, "-c", code], cwd=_build.ROOT).returncode == 0
+
+
+def test_no_source_names_a_multicast_qualifier():
+    """The kernels run on 1 to 8 GPUs; the peers of a cluster are signalled one by one, and a scan of the sources for the qualifier finds nothing."""
+    import re
+
+    sources = [p for folder in (_build.CSRC, _build.ROOT / "include") for p in folder.iterdir() if p.suffix in (".cu", ".cuh", ".h", ".cpp")]
+    assert len(sources) >= 12
+    assert [p.name for p in sources if re.search(r"multicast:{2}", p.read_text())] == []
