@@ -336,7 +336,7 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
                         umma_f8(tmem_base + out.idx * L::kSlotColumns + d * L::kWidth, L::kTokenLanes ? desc_a : desc_w, L::kTokenLanes ? desc_w : desc_a, p.idesc, k != 0 ? 1u : 0u);
                     }
                 }
-                umma_commit(&empty[slot.idx]);
+                if (i + L::kStages < steps) umma_commit(&empty[slot.idx]);   // no arrival that nobody waits for: the CTA might be gone by then
                 umma_commit(&tmem_full[out.idx]);
                 slot.advance(L::kStages);
                 out.advance(L::kSlots);
@@ -583,6 +583,10 @@ constexpr int kPairN = 256;
 constexpr int kPairEpilogueWarps = 8;                              // [half][lane quarter]
 constexpr int kPairThreads = 32 * (4 + kPairEpilogueWarps);        // warps 0-3: load, multiply h = 0 and 1, scales
 constexpr int kImageBytes = 32 * 64;                               // 32 rows x 32 outputs of 16 bits
+// Registers a thread, out of the 168 that a CTA of 384 threads starts with. With 56 for the first four warps the issuers and the scale warp spill (52 bytes
+// stored and 48 loaded, 4 and 12 with 64; 4096 x 4096 x 4096 77.6 us, 76.0 with 64, both in a sustained loop), 72 spill as much as 64.
+constexpr int kPairOtherRegisters = 64, kPairEpilogueRegisters = 216;
+static_assert(4 * kPairOtherRegisters + kPairEpilogueWarps * kPairEpilogueRegisters <= (4 + kPairEpilogueWarps) * 168, "an increase would wait for good");
 
 struct PairSmem {
     static constexpr int kStageBytes = 2 * kTileBytes;             // this CTA's 128 activation rows and its half of the outputs
@@ -648,7 +652,9 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     constexpr int seg = half_n / 2;      // of these, the ones in one UMMA group
 
     if (warp < 4) {
-        registers_decrease<56>();
+        registers_decrease<kPairOtherRegisters>();
+        // k blocks of all tiles of this pair
+        const uint32_t turns = first_tile < num_tiles ? static_cast<uint32_t>((num_tiles - 1 - first_tile) / tile_step + 1) * static_cast<uint32_t>(p.num_kb) : 0u;
         if (warp == 0 && elect_one()) {
             // ------------------------------------------------------------------ loads (this CTA's halves)
             grid_dependency_wait();
@@ -679,8 +685,9 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             grid_dependency_wait();
             Ring slot, out;
             bool ok = true;
+            uint32_t left = turns;
             for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
-                for (int kb = 0; kb < p.num_kb; ++kb) {
+                for (int kb = 0; kb < p.num_kb; ++kb, --left) {
                     // backward the weight box is MN-major: the group's outputs are bytes h * seg .. of its 128-byte rows
                     const uint32_t a_addr = smem_u32(smem + slot.idx * L::kStageBytes);
                     const uint32_t w_addr = a_addr + kTileBytes + h * (kBackward ? seg : seg * 128);
@@ -694,8 +701,10 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     }
 #pragma unroll
                     for (uint32_t dst = 0; dst < 2; ++dst) umma_commit_pair(map_to_cta(smem_u32(&tmem_full[2 * h + out.idx]), dst));
+                    if (left > kPairStages) {   // no arrival that nobody waits for: the CTA might be gone by then
 #pragma unroll
-                    for (uint32_t dst = 0; dst < 2; ++dst) umma_commit_pair(map_to_cta(smem_u32(&load_empty[slot.idx]), dst));
+                        for (uint32_t dst = 0; dst < 2; ++dst) umma_commit_pair(map_to_cta(smem_u32(&load_empty[slot.idx]), dst));
+                    }
                     slot.advance(kPairStages);
                     out.advance(2);
                 }
@@ -748,7 +757,6 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             grid_dependency_wait();
             enter();
             for (uint32_t i = 0; i < kScaleAhead; ++i) fetch(i);
-            const uint32_t turns = first_tile < num_tiles ? static_cast<uint32_t>((num_tiles - 1 - first_tile) / tile_step + 1) * static_cast<uint32_t>(p.num_kb) : 0u;
             for (uint32_t turn = 0; turn < turns; ++turn) {
                 cp_async_wait<kScaleAhead - 1>();
                 __syncwarp();
@@ -772,7 +780,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             cp_async_wait<0>();
         }
     } else {
-        registers_increase<216>();
+        registers_increase<kPairEpilogueRegisters>();
         // ---------------------------------------------------------------------- epilogue: this CTA's 128 rows
         const int quarter = warp % 4;
         const int half = (warp - 4) / 4;

@@ -92,3 +92,16 @@ def test_a_cta_that_gave_up_takes_its_cluster_along():
     told = body.find("if (warp == 0 && lane < splits && guard.aborted()) st_shared_cluster_u32(map_to_cta(smem_u32(tmem_slot + 1), static_cast<uint32_t>(lane)), 1u);")
     assert -1 < told < barrier < look
     assert "__syncthreads(); if (splits > 1) {" in body[told - 60 : told]   # every warp of this CTA has set the flag by then, if it does
+
+
+@pytest.mark.parametrize("kernel,barrier,condition", [("small_kernel", "empty", "i + L::kStages < steps"), ("pair_kernel", "load_empty", "left > kPairStages")])
+def test_no_commit_that_nobody_waits_for(kernel, barrier, condition):
+    """A commit arrives on its own. Where nobody waits for it, the arrival may come when the CTA (for a pair: the peer) has ended and its shared
+    memory is another one's. The loader waits for a stage's release before it fills the stage again: for all of them but those of the last round."""
+    body = re.sub(r"\s+", " ", kernels("fp8_block_mm_sm100.cu")[kernel][1])
+    commits = [m.start() for m in re.finditer(r"umma_commit(_pair)?\([^;]*[&(]" + barrier + r"\[", body)]
+    assert len(commits) == 1
+    assert f"if ({condition})" in body[commits[0] - 140 : commits[0]]
+    stages, steps = 4, 11
+    waited = [i - stages for i in range(steps) if i >= stages]      # the fill of step i waits for the release of step i - stages
+    assert [i for i in range(steps) if i + stages < steps] == [i for i in range(steps) if steps - i > stages] == waited
