@@ -86,7 +86,7 @@ def dequantize_fp8_weight(q: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
 
 def quantize_fp8_activation(x: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> tuple[torch.Tensor, torch.Tensor]:
     """Codes and block scales of a `[M, K]` fp16/bf16 activation, in one kernel: with `t` the largest magnitude of a block
-    (at least `1e-30 * top`), `scale = t / top` and `q = fp8(x * (top / t))`, in float32. Returns `(q [M, K], scale [ceil(K / 128), M])`."""
+    (at least `1e-30 * top`), `scale = t * (1 / top)` and `q = fp8(x * (top * (1 / t)))`, each step rounded to float32. Returns `(q [M, K], scale [ceil(K / 128), M])`."""
     return _ops.fp8_block_quantize.default(x, _is_e5m2(dtype))
 
 

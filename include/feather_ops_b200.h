@@ -148,8 +148,8 @@ int feather_conv3x3_launch(const void* x, const void* wp, const void* bias, void
 int feather_conv3x3_status(uint32_t* out);
 
 /* fp8 codes of an activation with one float32 scale per row and 128 channels: with t = max(max |x| over the block, 1e-30 top) and
- * top = 448 (e4m3) or 57344 (e5m2), scale = t / top and q = fp8(x * (top / t)). x: [M, K] fp16 (input_fp16 != 0) or bf16; q: [M, K];
- * scale: [ceil(K / 128), M]. K % 16 == 0, x and q 16-byte aligned. No counterpart in the reference (its quantizer is per row, to int8,
+ * top = 448 (e4m3) or 57344 (e5m2), scale = t * (1 / top) and q = fp8(x * (top * (1 / t))), each step rounded to float32. x: [M, K]
+ * fp16 (input_fp16 != 0) or bf16; q: [M, K]; scale: [ceil(K / 128), M]. K % 16 == 0, x and q 16-byte aligned. No counterpart in the reference (its quantizer is per row, to int8,
  * csrc/hip_kernel_int8.cu:869-878). */
 bool launch_fp8_block_quantize(const void* x, void* q, float* scale, int64_t M, int64_t K, int input_fp16, int use_e5m2, feather_stream_t stream);
 

@@ -142,3 +142,22 @@ def test_oracles_of_the_quantizer_agree(dtype):
     codes, scale = ofb.quantize(x.double(), dtype)
     assert ((s.double() - scale).abs() <= 2**-23 * scale).all()
     assert ((q.double() - codes).abs() <= ofb.half_step(codes, dtype) * (1 + 2**-18)).all()
+
+
+@pytest.mark.parametrize("dtype", [E4M3, E5M2])
+def test_the_documented_formula_gives_the_oracles_bits(dtype):
+    """`quantize_f32` are the steps that the quantizer is tested against bit for bit on a device: what is documented has to be those."""
+    import pathlib
+    import re
+
+    header = (pathlib.Path(__file__).resolve().parents[1] / "include" / "feather_ops_b200.h").read_text()
+    x = torch.randn(64, 128, generator=torch.Generator().manual_seed(5)).to(torch.bfloat16)
+    q_ref, s_ref = ofb.quantize_f32(x, dtype)
+    top = torch.tensor(ofb.TOP[dtype])
+    names = {"t": x.float().abs().amax(1), "top": top, "fp8": lambda v: v.to(dtype)}
+    for text in (fo.quantize_fp8_activation.__doc__, header[: header.index("launch_fp8_block_quantize(")]):
+        scale = re.search(r"scale = ([^`,\n]*?)(?:`| and)", text)[1]
+        code = re.search(r"\bq = (fp8\([^`,\n]*\))", text)[1].replace("x *", "x.float() *")
+        assert torch.equal(eval(scale, dict(names)), s_ref[0])
+        codes = [eval(code, names | {"x": x[i], "t": names["t"][i]}) for i in range(x.shape[0])]
+        assert torch.equal(torch.stack([c.view(torch.uint8) for c in codes]), q_ref.view(torch.uint8))
