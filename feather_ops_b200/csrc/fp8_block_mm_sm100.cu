@@ -77,15 +77,6 @@ __device__ __forceinline__ float bits_to_float(uint16_t v) {
 }
 
 template <bool kOutBf16>
-__device__ __forceinline__ uint16_t float_to_bits(float v) {
-    if constexpr (kOutBf16) {
-        return __bfloat16_as_ushort(__float2bfloat16_rn(v));
-    } else {
-        return __half_as_ushort(__float2half_rn(v));
-    }
-}
-
-template <bool kOutBf16>
 __device__ __forceinline__ uint32_t pack_out(float a, float b) {
     if constexpr (kOutBf16) {
         const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);

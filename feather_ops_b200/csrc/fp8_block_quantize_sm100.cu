@@ -521,7 +521,7 @@ struct RowShape {
     int threads, rows, chunks;   // blockDim.x, blockDim.y
 };
 
-constexpr int kSms = 148;   // of a B200
+constexpr int kSms = 148;   // of a B200: a constant, since the scratch's size is asked for without a device too
 
 RowShape row_shape(int64_t M, int64_t K) {
     const int64_t vectors = K / kVec;

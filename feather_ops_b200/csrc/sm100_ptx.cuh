@@ -159,7 +159,6 @@ __device__ __forceinline__ void cp_async_4(uint32_t smem_dst, const void* src, b
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_dst), "l"(src), "r"(src_bytes) : "memory");
 }
 
-
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
 template <int kPending>
