@@ -1,4 +1,4 @@
-"""Per-operator measurements: every operator of the library at its benchmark shapes, with vendor-library comparators.
+"""Per-operator measurements: every operator of the library at its benchmark shapes, with comparators where a vendor library has the like.
 
     python -m feather_ops_b200.benchmarks [scaled_mm] [msweep] [int8] [conv] [grid] [fp8_block] [cells] [--profile] [--peaks FILE]
 
@@ -496,8 +496,19 @@ def bench_cells(device, peaks, groups=None) -> list[dict]:
 # ------------------------------------------------------------------------------------------------------------- fp8_block
 # (tokens, N, K) of a product; the row-wise operators run on (rows, width)
 FP8_BLOCK_PRODUCTS = [(1, 12288, 4096), (24, 5120, 5120), (512, 4096, 4096), (1024, 4096, 4096), (4096, 4096, 4096), (8192, 12288, 4096)]
-FP8_BLOCK_ROWS = [(1, 4096), (333, 2576), (8192, 4096)]
+FP8_BLOCK_ROWS = [(1, 4096), (333, 2576), (8192, 4096), (4096, 16384), (4096, 32768)]
 FP8_BLOCK_GATES = [(1, 12288), (4096, 12288)]
+
+
+def _vendor_fp8_us(codes, weights) -> float | None:
+    """Microseconds of the vendor library's fp8 GEMM (`torch._scaled_mm`: one scale for each side, bf16 output) on the same codes. None if the
+    private entry point is missing or refuses the shape."""
+    try:
+        one = torch.ones((), device=codes[0][0].device)
+        sets = len(codes)
+        return time_launches(lambda i: torch._scaled_mm(codes[i % sets][0], weights[i % sets][0].t(), scale_a=one, scale_b=one, out_dtype=torch.bfloat16), sets)["us"]
+    except Exception:  # noqa: BLE001
+        return None
 
 
 def bench_fp8_block(device, peaks) -> list[dict]:
@@ -511,9 +522,9 @@ def bench_fp8_block(device, peaks) -> list[dict]:
     def rows_of(m, k):
         return torch.randn((m, k), device=device).to(torch.bfloat16)
 
-    def case(name, launch, sets, algorithmic_bytes, flop=None, bound="hbm"):
+    def case(name, launch, sets, algorithmic_bytes, flop=None, bound="hbm", **beside):
         timing = time_launches(launch, sets)
-        records.append(_rates({"case": name, "cold": True}, timing, flop=flop, algorithmic_bytes=algorithmic_bytes, bound=bound, peaks=peaks, int8=flop is not None))
+        records.append(_rates({"case": name, "cold": True, **beside}, timing, flop=flop, algorithmic_bytes=algorithmic_bytes, bound=bound, peaks=peaks, int8=flop is not None))
 
     for m, n, k in FP8_BLOCK_PRODUCTS:
         flop, traffic = 2.0 * m * n * k, n * k + m * k + 2 * m * n
@@ -523,7 +534,8 @@ def bench_fp8_block(device, peaks) -> list[dict]:
         inputs = [rows_of(m, k) for _ in range(sets)]
         codes = [fb.quantize_fp8_activation(x) for x in inputs]
         grads = [fb.quantize_fp8_activation(rows_of(m, n)) for _ in range(sets)]
-        case(f"fp8_block_mm {m}x{n}x{k}", lambda i: fb.fp8_block_mm(*codes[i % sets], *weights[i % sets]), sets, traffic, flop, bound)
+        vendor = {"vendor_same_shape_us": _round(_vendor_fp8_us(codes, weights), 2), "vendor_same_shape": "torch._scaled_mm on the same codes, one scale for each side"}
+        case(f"fp8_block_mm {m}x{n}x{k}", lambda i: fb.fp8_block_mm(*codes[i % sets], *weights[i % sets]), sets, traffic, flop, bound, **vendor)
         case(f"fp8_block_mm transposed {m}x{n}x{k}", lambda i: fb.fp8_block_mm(*grads[i % sets], *weights[i % sets], transposed_b=True), sets,
              n * k + m * n + 2 * m * k, flop, bound)
         case(f"fp8_block_linear {m}x{n}x{k}", lambda i: fb.fp8_block_linear(inputs[i % sets], *weights[i % sets]), sets, traffic + m * k, flop, bound)
@@ -535,6 +547,8 @@ def bench_fp8_block(device, peaks) -> list[dict]:
         case(f"quantize_fp8_activation {m}x{k}", lambda i: fb.quantize_fp8_activation(x[i % sets]), sets, 3 * m * k)
         case(f"rms_norm_quantize_fp8 residual {m}x{k}", lambda i: fb.rms_norm_quantize_fp8(x[i % sets], w, r[i % sets]), sets, 7 * m * k)
         case(f"rms_norm_dgrad residual {m}x{k}", lambda i: fb.rms_norm_dgrad(x[i % sets], r[i % sets], w, rstd, x[(i + 1) % sets]), sets, 8 * m * k)
+        wide = w.float()
+        case(f"rms_norm_dgrad residual, float32 weight {m}x{k}", lambda i: fb.rms_norm_dgrad(x[i % sets], r[i % sets], wide, rstd, x[(i + 1) % sets]), sets, 8 * m * k)
     for m, f in FP8_BLOCK_GATES:
         sets = sets_for(5 * m * f, True)
         gate_up, g = [rows_of(m, 2 * f) for _ in range(sets)], [rows_of(m, f) for _ in range(sets)]

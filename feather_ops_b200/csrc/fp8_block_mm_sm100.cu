@@ -11,10 +11,11 @@
 // Two kernels, picked by `launch`:
 //   * small_kernel: 128 outputs x 16, 32 or 128 tokens per CTA; for up to 32 tokens the weight is the M side of the UMMA,
 //     so that a few tokens cost no padding to 128 rows. K is split over the CTAs of a cluster, which add their partial sums through
-//     distributed shared memory in a fixed order. Bound by the weight's way from HBM and, at these sizes, by what a launch, the first
-//     loads and the exchange take: 1 x 12288 x 4096 12.7 us (50 MB, 4.0 TB/s), 512 x 4096 x 4096 14.1.
-//   * pair_kernel: 256 tokens x 256 outputs per CTA pair, persistent. 8192 x 12288 x 4096 386 to 405 us as the power cap allows
-//     (2.1 PFLOP/s), 4096 x 4096 x 4096 65 in bursts, 77 in a sustained loop under that cap.
+//     distributed shared memory in a fixed order. Bound by the pace of a CTA's k blocks (0.28 to 0.33 us each whatever their bytes) and, at these sizes,
+//     by what a launch, the first loads and the exchange take: 1 x 12288 x 4096 12.1 to 12.6 us (50 MB, 4.0 TB/s; the weight alone is 7.8 from HBM, and with
+//     the weight in L2 it takes 9.6), 24 x 5120 x 5120 10.5, 512 x 4096 x 4096 14.7.
+//   * pair_kernel: 256 tokens x 256 outputs per CTA pair, persistent. 8192 x 12288 x 4096 397 to 410 us as the power cap allows
+//     (2.0 PFLOP/s), 4096 x 4096 x 4096 68 in bursts of four launches, 75 to 76 in a sustained loop under that cap.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -116,7 +117,7 @@ __device__ __forceinline__ void let_copies_land(const WaitGuard& guard) {
 // brings the scales of k block after k block into shared memory with asynchronous copies, some blocks early, and writes the products
 // sa * sw for the epilogue warps. Its arrival is the second one on the accumulator's "full" barrier, so the epilogue waits for both
 // at once. It has to be quick: four-byte accesses, and its own next copies issued before the arrival, set the pace of both
-// kernels (4096 x 4096 x 4096 69.6 us, 64.9 now and 63.2 without scales; 512 x 4096 x 4096 15.3, 14.1 and 13.8).
+// kernels (4096 x 4096 x 4096 69.6 us, then 64.9, and 63.2 without scales; 512 x 4096 x 4096 15.3, 14.1 and 13.8).
 constexpr int kScaleAhead = 6;
 constexpr int kScaleRing = 8;   // raw scales: more than kScaleAhead, a lane may still read the one before
 
@@ -183,8 +184,9 @@ __device__ __forceinline__ void quantize_passes(const uint4 (&in)[kQuantizePasse
 // in three K splits 13.0 us against 10.9.)
 // Loads, UMMAs and accumulators are handed over in steps: two k blocks each up to 32 tokens, where a hand-over costs as much as the
 // block's UMMAs (1 x 12288 x 4096 12.7 us, 13.4 with one; 24 x 12288 x 4096 backward without a K split 23.0 and 24.7 at the time), one with 128 tokens (128 x 4096 x 4096
-// 11.0, 11.4 with two; 888 x 2352 x 992 7.6 and 7.9). What is left at 16 x 12288 x 4096: 12.4 us, of which HBM needs 7.8 for the
-// weight and the launch, the first loads and the drain some 3.5 (9.6 us with the weight in L2). Tiles of fewer outputs on more SMs take as long.
+// 11.0, 11.4 with two; 888 x 2352 x 992 7.6 and 7.9). What is left at 16 x 12288 x 4096: 12.1 us, 9.6 with the weight in
+// L2 (HBM would need 7.8 for it): 32 k blocks on each of 96 CTAs at their own pace, and launch, first loads and drain. Tiles of fewer outputs on more SMs, with as
+// many k blocks each, take as long.
 template <int T, bool kQuantize>
 struct SmallShape {
     static constexpr bool kTokenLanes = T == 128;
@@ -565,7 +567,7 @@ small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
 // h * seg .. of both CTAs' weight boxes), each with two accumulators, barriers and four epilogue warps of its own: the warps of one
 // half load accumulators from tensor memory while those of the other scale theirs. A k block takes some 700
 // clocks, and the tensor core works 62 % of them (4096 x 4096 x 4096): UMMAs and commit behind those of the other half, load, scale and release by the
-// epilogue, and the issuer's wait form a ring of two accumulators. At 4096 x 4096 x 4096 (64.5 us) a quarter of the UMMAs would save 8 us, no
+// epilogue, and the issuer's wait form a ring of two accumulators. At 4096 x 4096 x 4096 (64.5 us then) a quarter of the UMMAs would save 8 us, no
 // loads 7, no scaling 5, all three together 15. Other groups: four of 64 outputs take 16 to 24 % longer (8192 x 12288 x 4096 486 us, 390
 // with two), one of 256 with one issuer 13 to 25 % (486). 16 epilogue warps: 18 % (half the registers, so loads and products take turns).
 // Tiles of 128 outputs with four accumulators: 25 % (82.3 against 65.7), and slower than small_kernel where that is picked (512 x 4096 x 4096 16.0, 14.0).

@@ -13,8 +13,9 @@
 // All kernels move a few bytes per element through HBM, so few instructions per element are left: at 6.5 TB/s an SM gets 4 to 13
 // elements per clock and issues 4 warp instructions, i.e. 10 to 30 instructions per element. A thread has 8 consecutive channels
 // (one 16-byte load, one 8-byte store of codes) as four float pairs for the packed fp32 arithmetic; 16 lanes hold one block, and
-// its maximum is four shuffles. Measured, inputs from HBM: quantizer 4096 x 12288 24.4 us (6.2 TB/s of 6.46 that a copy reaches), gate
-// 4096 x 12288 39.2 (6.4), its backward pass 73.4 (6.9), norm 8192 x 4096 with a residual 38.5 (6.1), its backward pass 50.4 (5.3).
+// its maximum is four shuffles. Measured, inputs from HBM: quantizer 8192 x 4096 16.6 us (6.1 TB/s of 6.46 that a copy reaches), gate
+// 4096 x 12288 41 to 44 (5.7 to 6.1), norm 8192 x 4096 with a residual 37.7 to 38.5 (6.2), its backward pass 50.3 (5.3). The gate's backward pass takes 72
+// at 4096 x 12288, which for its 503 MB is above a copy's rate: a quarter of what it writes is still in L2 when it ends.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -279,7 +280,9 @@ struct NormGradParams {
 // CTA; a second kernel adds those in CTA order (the same bits on every run). A row is a chain of latencies (loads, ten shuffles, a
 // barrier), so what counts is how many rows an SM has on their way: two per CTA with the next row in registers (kAhead), else, at 64 registers, four CTAs
 // of 256 threads. (Copying the next rows to shared memory ahead of time was slower at the two or three CTAs that fit then: 68 to 75 us at
-// 8192 x 4096 with a residual, and so was every variant whose registers spill.)
+// 8192 x 4096 with a residual, and so was every variant whose registers spill there.) Above 16384 channels 1024 threads have four chunks each and the registers do
+// spill (460 bytes stored and 400 loaded a thread, 924 and 864 with a float32 weight): 4096 x 32768 with a residual 352 us and 522 to 608, where the bytes take 166;
+// 4096 x 16384 106 and 110 (83).
 template <bool kFp16, bool kWeightF32, int kChunks, int kThreads, bool kAhead>
 __global__ void __launch_bounds__(kThreads) rms_norm_dgrad_kernel(const NormGradParams p) {
     __shared__ float slots[2][32];
