@@ -4,6 +4,8 @@ The results are those of the same call on inputs that were there long before, bi
 the call's kernels has a limit of two seconds, which must not begin before the kernel ahead has finished.
 """
 
+import threading
+
 import pytest
 import torch
 
@@ -117,3 +119,77 @@ def test_linear_behind_a_kernel_of_some_seconds(cuda_device):
 @pytest.mark.parametrize("plain", [False, True], ids=["prepack", "plain"])
 def test_int8_product_behind_a_kernel_of_some_seconds(cuda_device, plain):
     late(*int8_product(plain), 0, LONG)
+
+
+@pytest.mark.parametrize("which", range(3), ids=["codes", "weight", "scales"])
+@pytest.mark.parametrize("plain", [False, True], ids=["prepack", "plain"])
+def test_int8_product_backward(cuda_device, plain, which):
+    n, k, m = 528, 1024, 2600
+    g = torch.Generator().manual_seed(3)
+    a, w = (torch.randint(-127, 128, s, generator=g, dtype=torch.int8).cuda() for s in ((m, n), (n, k)))
+    call = fo.int8_scaled_mm_plain if plain else fo.int8_scaled_mm
+    late(lambda *t: call(*t, transposed_b=True), (a, w if plain else fo.prepack_int8_weight(w), torch.rand(m, generator=g).cuda()), which, SHORT)
+
+
+def chain():
+    """A function of two matrices that runs every operator that starts early, each behind another one."""
+    w1, w2 = (fo.quantize_fp8_weight(rand(*s, seed=i, dtype=torch.float32, size=0.05)) for i, s in enumerate(((1056, 400), (400, 528))))
+    norm_weight = rand(400, seed=4)
+
+    def run(x, r):
+        q, s, h, rstd = fo.rms_norm_quantize_fp8(x, norm_weight, r)
+        gate_up = fo.fp8_block_mm(q, s, *w1)
+        y = fo.fp8_block_mm(*fo.silu_mul_quantize_fp8(gate_up), *w2)
+        d_gate_up = fo.silu_mul_dgrad(fo.fp8_block_dgrad(y, *w2), gate_up)
+        return h, gate_up, y, d_gate_up, *fo.rms_norm_dgrad(fo.fp8_block_linear(d_gate_up[:, :400].contiguous(), *w1)[:, :400].contiguous(), h, norm_weight, rstd)
+
+    return run, w1
+
+
+@pytest.mark.parametrize("m", [1, 30, 300, 1200])
+def test_captured_among_copies_fills_forks_and_joins(cuda_device, m):
+    run, w = chain()
+    x, r = rand(m, 400, seed=5), rand(m, 400, seed=6)
+    expected, swapped = run(x, r), run(r, x)
+    linear = fo.fp8_block_linear(x, *w)
+    xs, rs = torch.zeros_like(x), torch.zeros_like(r)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        xs.copy_(x)
+        rs.copy_(r)
+        here = run(xs, rs)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            there = run(rs, xs)
+        apart = fo.fp8_block_linear(xs, *w)
+        torch.cuda.current_stream().wait_stream(side)
+        joined = fo.fp8_block_linear(xs, *w)   # behind two kernels
+        xs.zero_()
+        zeros = fo.quantize_fp8_activation(xs)[0]
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip((*here, *there, apart, joined), (*expected, *swapped, linear, linear)))
+        assert not zeros.view(torch.uint8).any()
+
+
+def test_from_several_threads(cuda_device):
+    run, _ = chain()
+    x, r = rand(300, 400, seed=5), rand(300, 400, seed=6)
+    expected = run(x, r), run(r, x)
+    torch.cuda.synchronize()
+    same = {}
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            got = [run(*((x, r), (r, x))[i % 2]) for _ in range(20)]
+        stream.synchronize()
+        same[i] = all(torch.equal(a, b) for results in got for a, b in zip(results, expected[i % 2]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert same == dict.fromkeys(range(6), True)
